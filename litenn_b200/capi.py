@@ -115,6 +115,45 @@ LLAMA_SYMBOLS = {
 LL_QKV, LL_O, LL_GU, LL_DOWN, LL_HEAD = 0, 1, 2, 3, 4
 LL_ATTN_NORM, LL_FFN_NORM, LL_FINAL_NORM = 0, 1, 2
 
+
+
+class KVCacheDesc(ctypes.Structure):
+    """Mirror of qmm_kv_cache (include/litenn_kv.h)."""
+    _fields_ = [("fmt", _i), ("kv_heads", _i), ("head_dim", _i), ("page_tokens", _i), ("n_pages", _i64), ("pool_dev", _vp)]
+
+
+class KVBatch(ctypes.Structure):
+    """Mirror of qmm_kv_batch: KVBatch(batch, table_width, page_table_ptr, kv_len_ptr, row_begin_ptr or 0, rows)."""
+    _fields_ = [("batch", _i), ("table_width", _i), ("page_table_dev", _vp), ("kv_len_dev", _vp), ("row_begin_dev", _vp),
+                ("rows", _i64)]
+
+
+class Rope(ctypes.Structure):
+    """Mirror of qmm_rope: Rope(dim, ROPE_PAIRS or ROPE_HALVES, inv_freq_ptr, gain)."""
+    _fields_ = [("dim", _i), ("layout", _i), ("inv_freq_dev", _vp), ("gain", ctypes.c_double)]
+
+
+class RopeScaling(ctypes.Structure):
+    """Mirror of qmm_rope_scaling."""
+    _fields_ = [("kind", _i), ("factor", ctypes.c_float), ("trained", ctypes.c_float), ("beta_fast", ctypes.c_float),
+                ("beta_slow", ctypes.c_float)]
+
+
+# include/litenn_kv.h
+_cache, _batch, _rope = ctypes.POINTER(KVCacheDesc), ctypes.POINTER(KVBatch), ctypes.POINTER(Rope)
+KV_SYMBOLS = {
+    "qmm_rope_frequencies": (_i, [_i, ctypes.c_double, _vp, ctypes.POINTER(RopeScaling), _vp,
+                                  ctypes.POINTER(ctypes.c_double)]),
+    "qmm_kv_pool_bytes": (_i, [_cache, ctypes.POINTER(_sz)]),
+    "qmm_kv_append": (_i, [_i, _cache, _batch, _rope, _i, _i, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i, _i64, _vp]),
+    "qmm_kv_read": (_i, [_i, _cache, _batch, _vp, _i64, _vp, _i64, _i, _vp]),
+    "qmm_kv_attention": (_i, [_i, _cache, _batch, _i, _vp, _i, _i64, _vp, _i, _i64, ctypes.c_float, _i, _vp, _vp]),
+}
+KV_F16 = 0
+KV_WORKSPACE_BYTES = 16 * 1024 * 1024
+ROPE_PAIRS, ROPE_HALVES = 0, 1
+ROPE_SCALE_NONE, ROPE_SCALE_LINEAR, ROPE_SCALE_YARN = 0, 1, 2
+
 _lib = None
 
 
@@ -127,7 +166,7 @@ def load() -> ctypes.CDLL:
                 f"{LIB_PATH} is missing: build it with `python -m litenn_b200.build` "
                 "(nvcc, sm_100a).  There is no CPU or PyTorch fallback for this path.")
         lib = ctypes.CDLL(LIB_PATH)
-        for name, (restype, argtypes) in {**SYMBOLS, **LLAMA_SYMBOLS}.items():
+        for name, (restype, argtypes) in {**SYMBOLS, **LLAMA_SYMBOLS, **KV_SYMBOLS}.items():
             fn = getattr(lib, name)
             fn.restype = restype
             fn.argtypes = argtypes
@@ -263,6 +302,61 @@ class Weight:
             self.destroy()
         except Exception:
             pass
+
+
+class KVCache:
+    """A paged key/value cache in caller-owned memory (include/litenn_kv.h): `pool_ptr` points at
+    ``kv_pool_bytes(...)`` bytes.  Pointers are device addresses, strides count elements."""
+
+    def __init__(self, fmt: int, kv_heads: int, head_dim: int, page_tokens: int, n_pages: int, pool_ptr: int,
+                 device: int = 0):
+        self.desc = KVCacheDesc(fmt, kv_heads, head_dim, page_tokens, n_pages, pool_ptr)
+        self.device = device
+        lib = load()
+        self._append, self._read, self._attend = lib.qmm_kv_append, lib.qmm_kv_read, lib.qmm_kv_attention
+
+    def append(self, batch: KVBatch, rope: Rope | None, heads: int, dtype: int, q_ptr: int, q_stride: int, k_ptr: int,
+               k_stride: int, v_ptr: int, v_stride: int, q_out_ptr: int, q_dtype: int, q_out_stride: int,
+               stream: int = 0) -> None:
+        """Rotates queries and keys by their positions and stores keys and values; `heads` 0 and `q_ptr` 0: no queries."""
+        rc = self._append(self.device, self.desc, batch, rope, heads, dtype, q_ptr, q_stride, k_ptr, k_stride, v_ptr, v_stride,
+                          q_out_ptr, q_dtype, q_out_stride, stream)
+        if rc:
+            check(rc)
+
+    def read(self, batch: KVBatch, k_ptr: int, k_stride: int, v_ptr: int, v_stride: int, dtype: int, stream: int = 0) -> None:
+        """The values that the cache holds for the batch's rows."""
+        rc = self._read(self.device, self.desc, batch, k_ptr, k_stride, v_ptr, v_stride, dtype, stream)
+        if rc:
+            check(rc)
+
+    def attend(self, batch: KVBatch, heads: int, q_ptr: int, q_dtype: int, q_stride: int, out_ptr: int, out_dtype: int,
+               out_stride: int, scale: float, window: int, workspace_ptr: int, stream: int = 0) -> None:
+        """Causal attention of the batch's rows over their pages; the workspace has KV_WORKSPACE_BYTES, zeroed once."""
+        rc = self._attend(self.device, self.desc, batch, heads, q_ptr, q_dtype, q_stride, out_ptr, out_dtype, out_stride,
+                          scale, window, workspace_ptr, stream)
+        if rc:
+            check(rc)
+
+
+def kv_pool_bytes(fmt: int, kv_heads: int, head_dim: int, page_tokens: int, n_pages: int) -> int:
+    out = ctypes.c_size_t()
+    check(load().qmm_kv_pool_bytes(KVCacheDesc(fmt, kv_heads, head_dim, page_tokens, n_pages, None), ctypes.byref(out)))
+    return out.value
+
+
+def rope_frequencies(dim: int, theta: float, factors=None, scaling: RopeScaling | None = None):
+    """(inv_freq float64 [dim / 2], gain) of rotary positions; `factors`: fp32 [dim / 2] divisors (rope_freqs.weight)."""
+    import numpy as np
+    out = np.empty(max(dim, 0) // 2, dtype=np.float64)
+    if factors is not None:
+        factors = np.ascontiguousarray(factors, dtype=np.float32)
+        if factors.shape != out.shape:
+            raise ValueError("one factor per pair of dimensions is required")
+    gain = ctypes.c_double()
+    check(load().qmm_rope_frequencies(dim, theta, None if factors is None else factors.ctypes.data, scaling,
+                                      out.ctypes.data, ctypes.byref(gain)))
+    return out, gain.value
 
 
 def dequantize_raw(fmt: int, payload_ptr: int, n: int, k: int, out_ptr: int, device: int = 0, stream: int = 0) -> None:

@@ -1,0 +1,548 @@
+"""The paged key/value cache on the GPU against 64-bit sums (tests/kv_ref.py): append, read, attention."""
+import dataclasses
+import math
+
+import numpy as np
+import pytest
+
+import kv_ref as ref
+from litenn_b200 import capi
+
+pytestmark = pytest.mark.gpu
+
+FMTS = [ref.Q4_0, ref.Q8_0, ref.F16]
+
+
+@pytest.fixture(scope="module", autouse=True)
+def device(qmm_lib):
+    import torch
+    assert torch.cuda.is_available()
+    torch.cuda.set_device(0)
+    capi.kernel_status(0)
+
+
+def torch_of(x, bf16=False):
+    import torch
+    t = torch.from_numpy(np.ascontiguousarray(x)).cuda()
+    return t.bfloat16() if bf16 else t
+
+
+def np_of(t):
+    return t.float().cpu().numpy()
+
+
+@dataclasses.dataclass
+class Paged:
+    """A pool with shuffled pages and sequences of given lengths; every byte that no append has written is 0xFF."""
+    fmt: int
+    kv_heads: int
+    hd: int
+    page: int
+    lens: list
+    spare: int = 2
+    seed: int = 0
+
+    def __post_init__(self):
+        import torch
+        rng = np.random.default_rng(self.seed)
+        self.width = max(1, max(-(-n // self.page) for n in self.lens))
+        used = sum(-(-n // self.page) for n in self.lens)
+        self.n_pages = used + self.spare
+        order = rng.permutation(self.n_pages)[:used].tolist()
+        table = np.full((len(self.lens), self.width), 2 ** 30, dtype=np.int32)  # what lies past a length is not read
+        for s, n in enumerate(self.lens):
+            for i in range(-(-n // self.page)):
+                table[s, i] = order.pop()
+        self.table = table
+        nbytes = capi.kv_pool_bytes(self.fmt, self.kv_heads, self.hd, self.page, self.n_pages)
+        self.pool = torch.full((nbytes,), 255, dtype=torch.uint8, device="cuda")
+        self.cache = capi.KVCache(self.fmt, self.kv_heads, self.hd, self.page, self.n_pages, self.pool.data_ptr())
+        self.table_dev = torch_of(table)
+        self.workspace = torch.zeros(capi.KV_WORKSPACE_BYTES, dtype=torch.uint8, device="cuda")
+        self.hold = []
+
+    def batch(self, rows, lens, total=None, single=False):
+        begin = torch_of(np.concatenate([[0], np.cumsum(rows)]).astype(np.int32))
+        length = torch_of(np.asarray(lens, dtype=np.int32))
+        self.hold += [begin, length]
+        return capi.KVBatch(len(lens), self.width, self.table_dev.data_ptr(), length.data_ptr(),
+                            0 if single else begin.data_ptr(), sum(rows) if total is None else total)
+
+    def fill(self, rng, k_scale=1.0):
+        """Appends random keys and values up to the lengths, without rotation; the values that the cache holds."""
+        rows = list(self.lens)
+        k = (rng.standard_normal((sum(rows), self.kv_heads, self.hd)) * k_scale).astype(np.float32)
+        v = rng.standard_normal((sum(rows), self.kv_heads, self.hd)).astype(np.float32)
+        kd, vd, w = torch_of(k), torch_of(v), self.kv_heads * self.hd
+        self.cache.append(self.batch(rows, rows), None, 0, 0, 0, 0, kd.data_ptr(), w, vd.data_ptr(), w, 0, 0, 0)
+        assert capi.kernel_status(0) == 0
+        cut = np.cumsum(rows)[:-1]
+        return np.split(ref.stored(k, self.fmt), cut), np.split(ref.stored(v, self.fmt), cut)
+
+    def attend(self, q, rows, lens, heads, bf16=False, out_bf16=False, window=0, single=False, scale=None, total=None):
+        import torch
+        qd = torch_of(q.reshape(len(q), -1), bf16)
+        out = torch.full((len(q), heads * self.hd), 7.0, device="cuda", dtype=torch.bfloat16 if out_bf16 else torch.float32)
+        self.cache.attend(self.batch(rows, lens, total, single), heads, qd.data_ptr(), int(bf16), heads * self.hd,
+                          out.data_ptr(), int(out_bf16), heads * self.hd, self.hd ** -0.5 if scale is None else scale, window,
+                          self.workspace.data_ptr())
+        assert capi.kernel_status(0) == 0
+        return np_of(out).reshape(len(q), heads, self.hd).astype(np.float64)
+
+
+def check_attention(p, rows, lens, heads, rng, bf16=False, out_bf16=False, window=0, single=False, q_scale=2.0, half=False):
+    ks, vs = p.fill(rng)
+    q = (rng.standard_normal((sum(rows), heads, p.hd)) * q_scale).astype(np.float32)
+    if bf16:
+        q = ref.bf16_round(q)
+    got = p.attend(q, rows, lens, heads, bf16, out_bf16, window, single)
+    at = 0
+    for s, (n, r) in enumerate(zip(lens, rows)):
+        if r == 0:
+            continue
+        want = ref.attention(q[at:at + r], ks[s], vs[s], n, p.hd ** -0.5, window)
+        bound = ref.attention_bound(q[at:at + r], ks[s], vs[s], p.hd ** -0.5, out_bf16, half)
+        err = np.abs(got[at:at + r] - want).max()
+        assert err <= bound, (s, n, r, err, bound)
+        at += r
+
+
+# ---- append and read ----------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("hd,heads,kv_heads,page,rope_dim,halves,bf16", [
+    (128, 8, 2, 16, 128, False, False), (128, 4, 4, 64, 64, True, True), (64, 3, 1, 32, 64, True, False),
+    (96, 6, 3, 48, 96, True, False), (96, 2, 1, 16, 34, False, True), (256, 2, 2, 128, 256, True, False),
+    (256, 4, 1, 16, 0, False, False), (64, 2, 2, 16, 8, True, True)])
+def test_append_stores_what_the_rules_say(fmt, hd, heads, kv_heads, page, rope_dim, halves, bf16):
+    import torch
+    rng = np.random.default_rng(hd + page)
+    rows, lens = [5, 0, 1, 40], [21, 7, 1, 140]
+    p = Paged(fmt, kv_heads, hd, page, lens)
+    before = p.pool.clone()
+    width = heads + 2 * kv_heads
+    qkv = rng.standard_normal((sum(rows) + 3, width, hd)).astype(np.float32) * 3  # three rows behind the last sequence
+    qkv[0, heads] = 0.0                       # a block of zeros
+    qkv[1, heads + kv_heads, :32] = np.where(np.arange(32) % 5, 1.0, -2.5)  # equals of both signs
+    if bf16:
+        qkv = ref.bf16_round(qkv)
+    x = torch_of(qkv.reshape(len(qkv), -1), bf16)
+    freq, gain = capi.rope_frequencies(rope_dim or 2, 10000.0)
+    freq_dev = torch_of(freq)
+    rope = capi.Rope(rope_dim, int(halves), freq_dev.data_ptr(), 1.25) if rope_dim else None
+    q_out = torch.full((len(qkv), heads * hd), 9.0, device="cuda", dtype=x.dtype)
+    at, item, stride = x.data_ptr(), x.element_size(), width * hd
+    b = p.batch(rows, lens, total=len(qkv))
+    p.cache.append(b, rope, heads, int(bf16), at, stride, at + heads * hd * item, stride, at + (heads + kv_heads) * hd * item,
+                   stride, q_out.data_ptr(), int(bf16), heads * hd)
+    k_out = torch.full((len(qkv), kv_heads * hd), 9.0, device="cuda")
+    v_out = k_out.clone()
+    p.cache.read(b, k_out.data_ptr(), kv_heads * hd, v_out.data_ptr(), kv_heads * hd, 0)
+    assert capi.kernel_status(0) == 0
+    pos = np.concatenate([np.arange(n - r, n) for n, r in zip(lens, rows)])
+    n = len(pos)
+    want_q = ref.rotate(qkv[:n, :heads], pos, freq, 1.25, rope_dim, halves)
+    want_k = ref.stored(ref.rotate(qkv[:n, heads:heads + kv_heads], pos, freq, 1.25, rope_dim, halves), fmt)
+    want_v = ref.stored(qkv[:n, heads + kv_heads:], fmt)
+    np.testing.assert_array_equal(np_of(q_out)[:n].reshape(want_q.shape), ref.bf16_round(want_q) if bf16 else want_q)
+    np.testing.assert_array_equal(np_of(k_out)[:n].reshape(want_k.shape), want_k.astype(np.float32))
+    np.testing.assert_array_equal(np_of(v_out)[:n].reshape(want_v.shape), want_v.astype(np.float32))
+    for t in (q_out, k_out, v_out):
+        assert (t[n:] == 9.0).all()           # rows behind the last sequence
+    # the bytes lie where the header says, and nothing else was written
+    tb = ref.tile_bytes(fmt, hd)
+    pool = p.pool.cpu().numpy().reshape(p.n_pages, kv_heads, page // 16, tb)
+    seq = np.repeat(np.arange(4), rows)
+    for i in rng.choice(n, 6, replace=False):
+        for h in range(kv_heads):
+            tile = pool[p.table[seq[i], pos[i] // page], h, pos[i] % page // 16]
+            for d in rng.choice(hd, 8, replace=False):
+                assert np.float32(ref.tile_value(tile, fmt, hd, True, pos[i] % 16, d)) == np.float32(want_k[i, h, d])
+                assert np.float32(ref.tile_value(tile, fmt, hd, False, pos[i] % 16, d)) == np.float32(want_v[i, h, d])
+    written = n * kv_heads * tb // 16
+    changed = int((p.pool != before).sum())
+    assert changed <= written and changed > written // 2
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("halves", [False, True])
+def test_queries_may_be_rotated_in_place(fmt, halves):
+    rng = np.random.default_rng(3)
+    heads, hd, n = 4, 128, 37
+    p = Paged(fmt, 2, hd, 16, [n])
+    qkv = rng.standard_normal((n, heads + 4, hd)).astype(np.float32)
+    x = torch_of(qkv.reshape(n, -1))
+    freq, gain = capi.rope_frequencies(hd, 5e5)
+    f = torch_of(freq)
+    at, stride = x.data_ptr(), (heads + 4) * hd
+    p.cache.append(p.batch([n], [n]), capi.Rope(hd, int(halves), f.data_ptr(), gain), heads, 0, at, stride, at + heads * hd * 4,
+                   stride, at + (heads + 2) * hd * 4, stride, at, 0, stride)
+    assert capi.kernel_status(0) == 0
+    got = np_of(x).reshape(qkv.shape)
+    np.testing.assert_array_equal(got[:, :heads], ref.rotate(qkv[:, :heads], np.arange(n), freq, gain, hd, halves))
+    np.testing.assert_array_equal(got[:, heads:], qkv[:, heads:])
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_single_tokens_and_a_prompt_leave_the_same_bytes(fmt):
+    import torch
+    rng = np.random.default_rng(4)
+    hd, kv, n, far = 128, 2, 35, 90000
+    x = torch_of(rng.standard_normal((n, 2 * kv * hd)).astype(np.float32))
+    freq, gain = capi.rope_frequencies(hd, 10000.0)
+    f = torch_of(freq)
+    rope, stride = capi.Rope(hd, 0, f.data_ptr(), gain), 2 * kv * hd
+    pools = []
+    for steps in ([n], [1] * n, [3] * 11 + [2]):
+        p = Paged(fmt, kv, hd, 64, [far + n], spare=0)
+        done = 0
+        for r in steps:
+            at = x.data_ptr() + done * stride * 4
+            p.cache.append(p.batch([r], [far + done + r], single=r == 1), rope, 0, 0, 0, 0, at, stride, at + kv * hd * 4, stride,
+                           0, 0, 0)
+            done += r
+        assert capi.kernel_status(0) == 0
+        pools.append(p.pool)
+    assert torch.equal(pools[0], pools[1]) and torch.equal(pools[0], pools[2])
+
+
+@pytest.mark.parametrize("fmt", [ref.Q4_0, ref.Q8_0])
+def test_values_that_no_block_holds(fmt):
+    """Infinities and NaN make their own block NaN, values past fp16's scales saturate, tiny ones vanish."""
+    import torch
+    hd = 64
+    v = np.ones((5, 1, hd), dtype=np.float32)
+    v[0, 0, 3] = np.inf
+    v[1, 0, 40] = np.nan
+    v[2, 0, :32] = 3e38
+    v[3, 0, :32] = 1e-9
+    v[4, 0, 5] = -1e30
+    p = Paged(fmt, 1, hd, 16, [5])
+    x = torch_of(v.reshape(5, hd))
+    b = p.batch([5], [5])
+    p.cache.append(b, None, 0, 0, 0, 0, x.data_ptr(), hd, x.data_ptr(), hd, 0, 0, 0)
+    out = torch.empty(2, 5, hd, device="cuda")
+    p.cache.read(b, out[0].data_ptr(), hd, out[1].data_ptr(), hd, 0)
+    assert capi.kernel_status(0) == 0
+    want = ref.stored(v, fmt).astype(np.float32)[:, 0]
+    np.testing.assert_array_equal(np_of(out)[0], want)
+    np.testing.assert_array_equal(np_of(out)[1], want)
+    assert np.isnan(want[0, :32]).all() and np.isfinite(want[0, 32:]).all() and np.isfinite(want[2:]).all()
+
+
+# ---- attention -----------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("hd,heads,kv_heads,page", [(128, 8, 1, 64), (128, 4, 4, 16), (64, 14, 2, 32), (96, 9, 3, 16),
+                                                    (256, 4, 2, 128), (128, 24, 1, 16)])
+def test_single_tokens(fmt, hd, heads, kv_heads, page):
+    lens = [1, 16, 17, 700, 2, 333]
+    p = Paged(fmt, kv_heads, hd, page, lens, seed=hd)
+    check_attention(p, [1] * 6, lens, heads, np.random.default_rng(hd + heads), single=True)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("rows,lens", [([3, 5, 1], [3, 70, 1]), ([9], [2500]), ([2, 0, 4], [31, 12, 64]), ([33], [33])])
+@pytest.mark.parametrize("window", [0, 1, 20])
+def test_several_rows_and_windows(fmt, rows, lens, window):
+    p = Paged(fmt, 2, 128, 32, lens, seed=len(rows))
+    check_attention(p, rows, lens, 6, np.random.default_rng(sum(lens)), window=window)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("bf16,out_bf16", [(True, False), (False, True), (True, True)])
+def test_types_of_rows(fmt, bf16, out_bf16):
+    lens = [100, 37]
+    p = Paged(fmt, 2, 128, 16, lens)
+    check_attention(p, [2, 3], lens, 8, np.random.default_rng(9), bf16, out_bf16)
+
+
+def test_many_sequences_of_few_tokens():
+    """More sequences than a CTA has threads: the list of tiles is found in several rounds."""
+    lens = [1 + i % 23 for i in range(300)]
+    p = Paged(ref.Q4_0, 1, 64, 16, lens)
+    check_attention(p, [1] * 300, lens, 2, np.random.default_rng(1), single=True)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_one_long_sequence_among_short_ones(fmt):
+    lens = [5, 9000, 1, 40]
+    p = Paged(fmt, 1, 128, 64, lens)
+    check_attention(p, [1] * 4, lens, 8, np.random.default_rng(2), single=True)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_rows_that_see_nothing_give_zeros(fmt):
+    """A sequence of length zero, and rows in front of a sequence's first token."""
+    rng = np.random.default_rng(5)
+    p = Paged(fmt, 1, 64, 16, [0, 3, 20])
+    ks, vs = p.fill(rng)
+    rows, lens = [2, 5, 1], [0, 3, 20]
+    q = rng.standard_normal((8, 2, 64)).astype(np.float32)
+    got = p.attend(q, rows, lens, 2)
+    want = np.concatenate([ref.attention(q[a:a + r], ks[s], vs[s], n, 0.125) for s, (a, r, n) in
+                           enumerate(zip([0, 2, 7], rows, lens))])
+    assert (got[:4] == 0).all()
+    np.testing.assert_allclose(got, want, atol=ref.attention_bound(q, ks[2], vs[2], 0.125, False) +
+                               ref.attention_bound(q, ks[1], vs[1], 0.125, False), rtol=0)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("rows", [1, 6])
+def test_what_a_row_does_not_see_does_not_reach_it(fmt, rows):
+    """NaN in a later token, in front of the window, behind the length: only the rows that see them."""
+    rng = np.random.default_rng(6)
+    n, hd, heads = 45, 128, 4
+    p = Paged(fmt, 1, hd, 16, [n])
+    k = rng.standard_normal((n, 1, hd)).astype(np.float32)
+    v = rng.standard_normal((n, 1, hd)).astype(np.float32)
+    for bad in (np.nan, np.inf):
+        v2, k2 = v.copy(), k.copy()
+        v2[n - 3, 0, 70] = bad     # token n - 3 is seen by the last three rows
+        k2[4, 0, 7] = np.nan       # in front of the window
+        v2[5, 0, 7] = bad
+        kd, vd = torch_of(k2), torch_of(v2)
+        p.cache.append(p.batch([n], [n]), None, 0, 0, 0, 0, kd.data_ptr(), hd, vd.data_ptr(), hd, 0, 0, 0)
+        q = rng.standard_normal((rows, heads, hd)).astype(np.float32)
+        got = p.attend(q, [rows], [n], heads, window=30)
+        sees = np.arange(n - rows, n) >= n - 3
+        assert np.isfinite(got[~sees]).all()
+        touched = [70] if fmt == ref.F16 else range(64, 96)
+        assert not np.isfinite(got[sees][:, :, touched]).any()
+        others = np.setdiff1d(np.arange(hd), touched)
+        kk, vv = ref.stored(k2, fmt), ref.stored(v2, fmt)
+        want = ref.attention(q, np.nan_to_num(kk), np.where(np.isfinite(vv), vv, 0), n, hd ** -0.5, 30)
+        bound = ref.attention_bound(q, np.nan_to_num(kk), np.where(np.isfinite(vv), vv, 0), hd ** -0.5, False)
+        assert np.abs(got - want)[:, :, others].max() <= bound
+        if (~sees).any():
+            assert np.abs(got - want)[~sees].max() <= bound
+
+
+def test_a_row_of_nothing_but_nan_is_nan():
+    rng = np.random.default_rng(7)
+    p = Paged(ref.Q4_0, 1, 64, 16, [700, 10])
+    p.fill(rng)
+    q = rng.standard_normal((2, 4, 64)).astype(np.float32)
+    q[0, 1, 5] = np.nan
+    got = p.attend(q, [1, 1], [700, 10], 4, single=True)
+    assert np.isnan(got[0, 1]).all() and np.isfinite(got[0, [0, 2, 3]]).all() and np.isfinite(got[1]).all()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_large_and_small_magnitudes(fmt):
+    """Scores of a hundred, values of 1e-4 beside values of 1e3, queries of 1e-6 and 1e6."""
+    rng = np.random.default_rng(8)
+    n, hd = 600, 64
+    p = Paged(fmt, 1, hd, 16, [n])
+    k = rng.standard_normal((n, 1, hd)).astype(np.float32) * 4
+    v = (rng.standard_normal((n, 1, hd)) * 10.0 ** rng.integers(-4, 4, (n, 1, 1))).astype(np.float32)
+    kd, vd = torch_of(k), torch_of(v)
+    p.cache.append(p.batch([n], [n]), None, 0, 0, 0, 0, kd.data_ptr(), hd, vd.data_ptr(), hd, 0, 0, 0)
+    kk, vv = ref.stored(k, fmt), ref.stored(v, fmt)
+    for size in (1e-6, 1.0, 8.0):
+        q = rng.standard_normal((1, 3, hd)).astype(np.float32) * np.float32(size)
+        got = p.attend(q, [1], [n], 3)
+        want = ref.attention(q, kk, vv, n, hd ** -0.5)
+        assert np.abs(got - want).max() <= ref.attention_bound(q, kk, vv, hd ** -0.5, False)
+
+
+def test_padding_rows_and_strided_rows_stay_as_they_were():
+    import torch
+    rng = np.random.default_rng(11)
+    p = Paged(ref.Q8_0, 2, 64, 16, [50, 9])
+    ks, vs = p.fill(rng)
+    rows, lens, heads, wide = [3, 1], [50, 9], 4, 4 * 64 + 24
+    q = rng.standard_normal((7, wide)).astype(np.float32)
+    qd = torch_of(q)
+    out = torch.full((7, wide), 5.0, device="cuda")
+    p.cache.attend(p.batch(rows, lens, total=7), heads, qd.data_ptr() + 32, 0, wide, out.data_ptr() + 64, 0, wide, 0.125, 0,
+                   p.workspace.data_ptr())
+    assert capi.kernel_status(0) == 0
+    o = np_of(out)
+    assert (o[4:] == 5.0).all() and (o[:, :16] == 5.0).all() and (o[:, 16 + 256:] == 5.0).all()
+    qq = q[:, 8:8 + 256].reshape(7, heads, 64)
+    want = np.concatenate([ref.attention(qq[:3], ks[0], vs[0], 50, 0.125), ref.attention(qq[3:4], ks[1], vs[1], 9, 0.125)])
+    assert np.abs(o[:4, 16:16 + 256].reshape(4, heads, 64) - want).max() <= ref.attention_bound(qq, ks[0], vs[0], 0.125, False)
+
+
+def test_same_inputs_same_bits_and_a_clean_workspace():
+    import torch
+    rng = np.random.default_rng(12)
+    lens = [3000, 800, 5]
+    p = Paged(ref.Q4_0, 2, 128, 64, lens)
+    p.fill(rng)
+    q = rng.standard_normal((3, 8, 128)).astype(np.float32)
+    first = p.attend(q, [1] * 3, lens, 8, single=True)
+    for _ in range(3):
+        np.testing.assert_array_equal(p.attend(q, [1] * 3, lens, 8, single=True), first)
+    # the first 16 KiB hold the counters that a call leaves zeroed
+    assert int(p.workspace[:16384].to(torch.int32).sum()) == 0
+
+
+def test_replayed_graph_follows_the_lengths():
+    """append + attend captured once: each replay appends one token more, on a stream of its own."""
+    import torch
+    rng = np.random.default_rng(13)
+    hd, heads, kv, n, steps = 128, 8, 2, 40, 6
+    p = Paged(ref.Q4_0, kv, hd, 16, [n + steps, 20 + steps])
+    full = rng.standard_normal((2, n + steps, 2 * kv, hd)).astype(np.float32)
+    freq, gain = capi.rope_frequencies(hd, 10000.0)
+    f = torch_of(freq)
+    rope = capi.Rope(hd, 0, f.data_ptr(), gain)
+    stride = (heads + 2 * kv) * hd
+    for s, m in enumerate([n, 20]):  # the prompts
+        x = torch_of(full[s, :m].reshape(m, -1))
+        b = p.batch([m], [m])
+        b.page_table_dev = p.table_dev[s].data_ptr()
+        p.cache.append(b, rope, 0, 0, 0, 0, x.data_ptr(), 2 * kv * hd, x.data_ptr() + kv * hd * 4, 2 * kv * hd, 0, 0, 0)
+    qkv = torch.zeros(2, stride, device="cuda")
+    length = torch.tensor([n, 20], device="cuda", dtype=torch.int32)
+    out = torch.zeros(2, heads * hd, device="cuda")
+    b = capi.KVBatch(2, p.width, p.table_dev.data_ptr(), length.data_ptr(), 0, 2)
+    at = qkv.data_ptr()
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def step():
+        length.add_(1)
+        p.cache.append(b, rope, heads, 0, at, stride, at + heads * hd * 4, stride, at + (heads + kv) * hd * 4, stride, at, 0,
+                       stride, stream.cuda_stream)
+        p.cache.attend(b, heads, at, 0, stride, out.data_ptr(), 0, heads * hd, hd ** -0.5, 0, p.workspace.data_ptr(),
+                       stream.cuda_stream)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(stream):
+        with torch.cuda.graph(graph, stream=stream):
+            step()
+    length.copy_(torch.tensor([n, 20]))
+    for i in range(steps):
+        q = rng.standard_normal((2, heads, hd)).astype(np.float32)
+        new = np.stack([full[0, n + i], full[1, 20 + i]])
+        torch.cuda.synchronize()
+        qkv.copy_(torch_of(np.concatenate([q, new], 1).reshape(2, -1)))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = np_of(out).reshape(2, heads, hd)
+        for s, m in enumerate([n + i + 1, 20 + i + 1]):
+            pos = np.arange(m)
+            keys = ref.stored(ref.rotate(full[s, :m, :kv], pos, freq, gain, hd, False), ref.Q4_0)
+            vals = ref.stored(full[s, :m, kv:], ref.Q4_0)
+            qr = ref.rotate(q[s:s + 1], pos[-1:], freq, gain, hd, False)
+            want = ref.attention(qr, keys, vals, m, hd ** -0.5)
+            assert np.abs(got[s] - want[0]).max() <= ref.attention_bound(qr, keys, vals, hd ** -0.5, False)
+    assert capi.kernel_status(0) == 0
+    del graph
+
+
+def test_two_calls_at_once_on_two_streams():
+    import torch
+    rng = np.random.default_rng(14)
+    caches = [Paged(ref.Q4_0, 2, 128, 64, [5000, 77], seed=i) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in caches]
+    data = [(p.fill(rng), rng.standard_normal((2, 8, 128)).astype(np.float32)) for p in caches]
+    qs = [torch_of(q.reshape(2, -1)) for _, q in data]
+    outs = [torch.zeros(2, 8 * 128, device="cuda") for _ in caches]
+    batches = [p.batch([1, 1], [5000, 77], single=True) for p in caches]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for p, s, q, o, b in zip(caches, streams, qs, outs, batches):
+            p.cache.attend(b, 8, q.data_ptr(), 0, 1024, o.data_ptr(), 0, 1024, 128 ** -0.5, 0, p.workspace.data_ptr(),
+                           s.cuda_stream)
+    torch.cuda.synchronize()
+    assert capi.kernel_status(0) == 0
+    for ((ks, vs), q), o in zip(data, outs):
+        for s, n in enumerate([5000, 77]):
+            want = ref.attention(q[s:s + 1], ks[s], vs[s], n, 128 ** -0.5)
+            assert np.abs(np_of(o)[s].reshape(8, 128) - want[0]).max() <= ref.attention_bound(q[s:s + 1], ks[s], vs[s],
+                                                                                              128 ** -0.5, False)
+
+
+def test_pool_past_32_bits():
+    """The last pages of a pool of more than 4 GiB."""
+    import torch
+    rng = np.random.default_rng(15)
+    hd, kv, page = 128, 8, 128
+    per_page = capi.kv_pool_bytes(ref.F16, kv, hd, page, 1)
+    n_pages = (5 << 30) // per_page
+    pool = torch.empty(n_pages * per_page, dtype=torch.uint8, device="cuda")
+    cache = capi.KVCache(ref.F16, kv, hd, page, n_pages, pool.data_ptr())
+    n = 200
+    table = torch.tensor([[n_pages - 1, n_pages - 2]], dtype=torch.int32, device="cuda")
+    length = torch.tensor([n], dtype=torch.int32, device="cuda")
+    begin = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    k, v = rng.standard_normal((2, n, kv, hd)).astype(np.float32)
+    kd, vd = torch_of(k), torch_of(v)
+    cache.append(capi.KVBatch(1, 2, table.data_ptr(), length.data_ptr(), begin.data_ptr(), n), None, 0, 0, 0, 0, kd.data_ptr(),
+                 kv * hd, vd.data_ptr(), kv * hd, 0, 0, 0)
+    q = rng.standard_normal((1, kv, hd)).astype(np.float32)
+    qd = torch_of(q)
+    out = torch.empty(1, kv * hd, device="cuda")
+    work = torch.zeros(capi.KV_WORKSPACE_BYTES, dtype=torch.uint8, device="cuda")
+    cache.attend(capi.KVBatch(1, 2, table.data_ptr(), length.data_ptr(), 0, 1), kv, qd.data_ptr(), 0, kv * hd, out.data_ptr(), 0,
+                 kv * hd, hd ** -0.5, 0, work.data_ptr())
+    assert capi.kernel_status(0) == 0
+    kk, vv = ref.stored(k, ref.F16), ref.stored(v, ref.F16)
+    want = ref.attention(q, kk, vv, n, hd ** -0.5)
+    assert np.abs(np_of(out).reshape(1, kv, hd) - want).max() <= ref.attention_bound(q, kk, vv, hd ** -0.5, False)
+
+
+# ---- what cannot be right is reported -------------------------------------------------------------------------------------
+
+def status_of(call):
+    call()
+    with pytest.raises(capi.QmmError) as e:
+        capi.kernel_status(0)
+    assert e.value.code == capi.E_KERNEL and capi.kernel_status(0) == 0
+    return str(e.value)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_bad_pages_and_rows_are_skipped_and_reported(fmt):
+    import torch
+    rng = np.random.default_rng(16)
+    p = Paged(fmt, 1, 64, 16, [40, 40])
+    ks, vs = p.fill(rng)
+    pool = p.pool.clone()
+    good = p.table_dev.clone()
+    x = torch_of(rng.standard_normal((4, 64)).astype(np.float32))
+    q = rng.standard_normal((2, 2, 64)).astype(np.float32)
+    qd, out = torch_of(q.reshape(2, -1)), torch.zeros(2, 128, device="cuda")
+
+    def append(b):
+        p.cache.append(b, None, 0, 0, 0, 0, x.data_ptr(), 64, x.data_ptr(), 64, 0, 0, 0)
+
+    def attend(b):
+        p.cache.attend(b, 2, qd.data_ptr(), 0, 128, out.data_ptr(), 0, 128, 0.125, 0, p.workspace.data_ptr())
+
+    for page in (-1, p.n_pages, 2 ** 31 - 1):
+        p.table_dev[0, 2] = page
+        assert "21" in status_of(lambda: append(p.batch([2, 0], [40, 40])))
+        assert "21" in status_of(lambda: attend(p.batch([1, 1], [40, 40], single=True)))
+        want = ref.attention(q[1:], ks[1], vs[1], 40, 0.125)  # the other sequence is as ever
+        assert np.abs(np_of(out)[1].reshape(2, 64) - want[0]).max() <= ref.attention_bound(q, ks[1], vs[1], 0.125, False)
+    p.table_dev.copy_(good)
+    for rows, lens, begin in (([1, 1], [49, 40], None), ([1, 1], [-1, 40], None), ([1, 1], [40, 40], [0, -5, 2]),
+                              ([1, 1], [40, 40], [0, 9, 2])):
+        b = p.batch(rows, lens)
+        if begin is not None:
+            t = torch.tensor(begin, dtype=torch.int32, device="cuda")
+            p.hold.append(t)
+            b.row_begin_dev = t.data_ptr()
+        assert "22" in status_of(lambda: attend(b))
+    assert "22" in status_of(lambda: append(p.batch([4], [3])))  # rows in front of the first token
+    assert torch.equal(p.pool, pool)
+    assert int(p.workspace[:16384].to(torch.int32).sum()) == 0
+    got = p.attend(q, [1, 1], [40, 40], 2, single=True)          # and the next call is whole
+    for s in range(2):
+        want = ref.attention(q[s:s + 1], ks[s], vs[s], 40, 0.125)
+        assert np.abs(got[s] - want[0]).max() <= ref.attention_bound(q, ks[s], vs[s], 0.125, False)
+
+
+def test_empty_calls_do_nothing():
+    p = Paged(ref.Q4_0, 1, 64, 16, [4])
+    b = capi.KVBatch(0, p.width, p.table_dev.data_ptr(), p.table_dev.data_ptr(), 0, 0)
+    p.cache.append(b, None, 0, 0, 0, 0, 0, 64, 0, 64, 0, 0, 0)
+    p.cache.read(b, 0, 64, 0, 64, 0)
+    p.cache.attend(b, 2, 0, 0, 128, 0, 0, 128, 0.125, 0, 0)
+    assert capi.kernel_status(0) == 0 and math.isfinite(1.0)
