@@ -369,7 +369,9 @@ int qmm_kv_attention(int device, const qmm_kv_cache* cache, const qmm_kv_batch* 
     a.scale = scale;
     a.window = window;
     a.workspace = static_cast<uint8_t*>(workspace_dev);
-    const cudaError_t e = launch_kv_attention(a, sm_count_of(device), static_cast<cudaStream_t>(stream));
+    const int sms = sm_count_of(device);
+    const cudaError_t e = kv_takes_prompt(a) ? launch_kv_prompt(a, sms, static_cast<cudaStream_t>(stream))
+                                             : launch_kv_rows(a, sms, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? QMM_OK : fail_cuda(e, who);
 }
 

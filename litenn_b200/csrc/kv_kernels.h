@@ -45,6 +45,12 @@ struct KvAttnArgs {
     int window;  // 0: none
     uint8_t* workspace;
 };
-cudaError_t launch_kv_attention(const KvAttnArgs& a, int sm_count, cudaStream_t stream);
+// Workspace: counters of the rows kernel, two of the prompt kernel, parts of the rows kernel's results.
+constexpr int KV_COUNTER_BYTES = 16384 - 64, KV_PARTS_AT = 16384;
+cudaError_t launch_kv_rows(const KvAttnArgs& a, int sm_count, cudaStream_t stream);
+// Long prompts with bf16 results (head_dim 64 or 128).
+cudaError_t launch_kv_prompt(const KvAttnArgs& a, int sm_count, cudaStream_t stream);
+// Whether a call goes to launch_kv_prompt.
+bool kv_takes_prompt(const KvAttnArgs& a);
 
 }  // namespace qmm

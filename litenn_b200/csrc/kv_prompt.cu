@@ -1,0 +1,777 @@
+// Attention of prompts over the paged cache on the 5th-generation tensor cores (include/litenn_kv.h), bf16 results.
+//
+// A CTA takes 256 columns of a kv head (query heads of its group, times rows) as two M tiles of 128, and walks the keys in
+// blocks of 128.  Per block and M tile:
+//   S = Q K^T   tcgen05.mma, both operands fp16 in shared memory, S fp32 in TMEM
+//   P           one thread per column: running maximum, exp2, sum; P in fp16 over S's own TMEM columns
+//   O += P V    tcgen05.mma, P from TMEM, V^T from shared memory, O fp32 in TMEM
+// Warps: 4 per M tile for the softmax (a warp reaches 32 TMEM lanes), 8 that bring keys and values (a tile of 16 tokens each,
+// from the cache to fp16 in swizzled shared memory, two stages), one that issues the MMAs.  While one M tile's softmax runs, the
+// tensor core works for the other.
+//
+// Numerics: queries are brought to fp16 by a power of two per row (11 bits below their largest), keys and values are the
+// cache's q * scale rounded to fp16 once, probabilities fp16 relative to a maximum that may lag 2^8 behind (O is scaled
+// only when it grows by more).  Each of the four roundings is 2^-12 of its value where the bf16 result's own is 2^-9.  Sums are
+// fp32.  A value that is not finite would reach every column of the product (0 times infinity): it enters as 0, and
+// the columns that see its token are made NaN.
+#include <algorithm>
+
+#include "kv_kernels.h"
+#include "kv_rows_plan.cuh"
+#include "qmm_gemm_ptx.cuh"
+
+#include "../../include/litenn_kv.h"
+
+namespace qmm {
+
+namespace {
+
+constexpr int BLOCK = 128;                     // keys per block
+constexpr int M_TILE = 128, COLS = 2 * M_TILE; // columns of an M tile, of a CTA
+constexpr int SOFT_WARPS = 8, KV_WARPS = 8;
+constexpr int THREADS = (SOFT_WARPS + KV_WARPS + 1) * 32;
+constexpr uint32_t TMEM_COLS = 512;            // S0, S1, O0, O1
+constexpr int KV_LATE_PROMPT = 24;             // a bounded wait ran out
+constexpr float SLACK = 8.0f;                  // how far the maximum may lag, in powers of two
+
+template <int FMT, int HD>
+struct PromptShape {
+    static constexpr int PANELS = HD / 64;                     // 64 dimensions: a 128-byte swizzle row
+    static constexpr int Q_BYTES = PANELS * M_TILE * 128;      // of an M tile
+    static constexpr int K_BYTES = PANELS * BLOCK * 128;       // of a stage
+    static constexpr int V_BYTES = BLOCK / 64 * HD * 128;
+    static constexpr int CONTROL = 4096;                       // barriers and what the warps tell one another
+    static constexpr int SMEM = 1024 + CONTROL + 2 * Q_BYTES + 2 * K_BYTES + 2 * V_BYTES;
+};
+
+struct Control {
+    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full;
+    uint32_t tmem;
+    int item_seq, item_local;
+    int late;
+    uint32_t poison[2][KV_WARPS];  // per stage and tile: tokens whose value is not finite
+    float q_scale[COLS];
+};
+
+// Instruction descriptor: D fp32, A and B fp16, both K-major, M = 128, N = n.
+__device__ __forceinline__ uint32_t idesc_f16(int n)
+{
+    return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(M_TILE >> 4) << 24);
+}
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add)
+{
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+        "}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        : "memory");
+}
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add)
+{
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+        "}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&r)[32])
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
+        "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]),
+          "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]), "=f"(r[17]), "=f"(r[18]),
+          "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]),
+          "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+        : "r"(addr)
+        : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const float (&r)[32])
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
+        "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+        "f"(r[0]), "f"(r[1]), "f"(r[2]), "f"(r[3]), "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7]), "f"(r[8]), "f"(r[9]), "f"(r[10]),
+        "f"(r[11]), "f"(r[12]), "f"(r[13]), "f"(r[14]), "f"(r[15]), "f"(r[16]), "f"(r[17]), "f"(r[18]), "f"(r[19]), "f"(r[20]),
+        "f"(r[21]), "f"(r[22]), "f"(r[23]), "f"(r[24]), "f"(r[25]), "f"(r[26]), "f"(r[27]), "f"(r[28]), "f"(r[29]), "f"(r[30]),
+        "f"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16])
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(
+            addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st()
+{
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void fence_before()
+{
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void fence_after()
+{
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ float exp2_fast(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t h2_bits(__half2 h)
+{
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ __half2 as_h2(uint32_t u)
+{
+    return *reinterpret_cast<const __half2*>(&u);
+}
+// Four pairs of a word's (two words', four words') values as exact fp16 quants, in storage order (kv_layout.cuh).
+template <int FMT>
+__device__ __forceinline__ void quants(const uint32_t* w, uint32_t (&v)[4])
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (FMT == FMT_Q4_0) {
+            const uint32_t x = i >= 2 ? w[0] >> 8 : w[0];
+            const uint32_t bits = (x & (i & 1 ? 0x00F000F0u : 0x000F000Fu)) | 0x64006400u;  // 1024 + n, or 1024 + 16 n
+            v[i] = i & 1 ? h2_bits(__hfma2(as_h2(bits), as_h2(0x2C002C00u), as_h2(0xD480D480u)))  // / 16 - 72
+                         : h2_bits(__hadd2(as_h2(bits), as_h2(0xE408E408u)));                      // - 1032
+        } else if (FMT == FMT_Q8_0) {
+            const uint32_t bits = __byte_perm(w[i >> 1], 0x64646464u, i & 1 ? 0x4342u : 0x4140u);  // 1024 + (q + 128)
+            v[i] = h2_bits(__hadd2(as_h2(bits), as_h2(0xE480E480u)));                              // - 1152
+        } else {
+            v[i] = w[i];
+        }
+    }
+}
+template <int BYTES>
+__device__ __forceinline__ void load_words(uint32_t* w, const uint8_t* p)
+{
+    if (BYTES == 16) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else {
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+        w[0] = v.x, w[1] = v.y;
+    }
+}
+
+// What a CTA works on: 256 columns of a kv head of a sequence.
+struct Item {
+    KvSeq q;
+    int seq, head;
+    int col0, cols;       // of the sequence's columns
+    int first_pos;        // of row 0
+    int k0;               // first key, a multiple of 16
+    int blocks[2], most;  // of each M tile
+    int pos_hi, seen_lo;  // keys that some column sees
+};
+
+template <int FMT, int HD>
+__global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs a)
+{
+    using Shape = PromptShape<FMT, HD>;
+    constexpr int NB = HD / 32, TILE = kv_tile_bytes(FMT, HD), PLANE = kv_plane_bytes(FMT, HD), SCALES = kv_scale_bytes(FMT, HD);
+    constexpr int U = kv_unit(FMT), LANE = kv_lane_bytes(FMT, HD), VEC = kv_vec(FMT, HD), VB = VEC / U;
+    constexpr bool QUANT = FMT != KV_F16;
+    extern __shared__ uint8_t prompt_smem[];
+    uint8_t* smem = prompt_smem + ((1024u - (g_smem_u32(prompt_smem) & 1023u)) & 1023u);
+    Control& ctl = *reinterpret_cast<Control*>(smem);
+    static_assert(sizeof(Control) <= Shape::CONTROL, "control block");
+    uint8_t* q_smem = smem + Shape::CONTROL;                 // [2 M tiles][panels][128 columns][128 B]
+    uint8_t* k_smem = q_smem + 2 * Shape::Q_BYTES;           // [2 stages][panels][128 keys][128 B]
+    uint8_t* v_smem = k_smem + 2 * Shape::K_BYTES;           // [2 stages][2 halves of the keys][HD rows][128 B]
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const bool mma_warp = warp == SOFT_WARPS + KV_WARPS;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            g_mbar_init(&ctl.k_full[i], KV_WARPS);
+            g_mbar_init(&ctl.v_full[i], KV_WARPS);
+            g_mbar_init(&ctl.k_empty[i], 1);
+            g_mbar_init(&ctl.v_empty[i], 1);
+            g_mbar_init(&ctl.s_full[i], 1);
+            g_mbar_init(&ctl.p_full[i], 4);
+        }
+        g_mbar_init(&ctl.o_full, 1);
+        ctl.late = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (mma_warp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(g_smem_u32(&ctl.tmem)), "r"(TMEM_COLS)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = ctl.tmem;
+    g_pdl_launch_dependents();
+    g_pdl_wait();
+
+    unsigned int* next_item = reinterpret_cast<unsigned int*>(a.workspace + KV_COUNTER_BYTES);
+    unsigned int* done_ctas = next_item + 1;
+    uint32_t blocks_before = 0, tile_before[2] = {0, 0}, items_before = 0;  // completed: the barriers' parities
+    auto give_up = [&]() {
+        atomicExch(a.seqs.status, KV_LATE_PROMPT);
+        *reinterpret_cast<volatile int*>(&ctl.late) = 1;
+    };
+
+    for (bool first = true;; first = false) {
+        // ---- the next item: heavy ones (late columns) of a sequence first, its kv heads side by side ----
+        if (mma_warp) {
+            unsigned int want = blockIdx.x;
+            if (!first) {
+                if (lane == 0) {
+                    want = gridDim.x + atomicAdd(next_item, 1u);
+                }
+                want = __shfl_sync(0xFFFFFFFFu, want, 0);
+            }
+            long long before = 0;
+            int seq = -1, local = 0;
+            for (int base = 0; base < a.seqs.batch && seq < 0; base += 32) {
+                const int s = base + lane;
+                bool bad = false;
+                long long n = 0;
+                if (s < a.seqs.batch) {
+                    const KvSeq q = kv_seq(a.pool, a.seqs, s, bad);
+                    n = ((long long)q.n * a.group + COLS - 1) / COLS * a.pool.kv_heads;
+                }
+                if (bad && blockIdx.x == 0 && first) {
+                    atomicExch(a.seqs.status, KV_BAD_ROWS);
+                }
+                long long upto = n;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const long long u = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+                    upto += lane >= o ? u : 0;
+                }
+                const bool mine = n > 0 && before + upto - n <= want && want < before + upto;
+                const unsigned int who = __ballot_sync(0xFFFFFFFFu, mine);
+                if (who != 0) {
+                    const int from = __ffs(who) - 1;
+                    seq = base + from;
+                    local = (int)(want - (before + __shfl_sync(0xFFFFFFFFu, upto - n, from)));
+                }
+                before += __shfl_sync(0xFFFFFFFFu, upto, 31);
+            }
+            if (lane == 0) {
+                ctl.item_seq = seq;
+                ctl.item_local = local;
+            }
+        }
+        __syncthreads();
+        if (ctl.item_seq < 0 || ctl.late) {
+            break;
+        }
+        Item it;
+        {
+            bool bad;
+            it.seq = ctl.item_seq;
+            it.q = kv_seq(a.pool, a.seqs, it.seq, bad);
+            const long long columns = (long long)it.q.n * a.group;
+            const int tiles = (int)((columns + COLS - 1) / COLS);
+            const int tile = tiles - 1 - ctl.item_local / a.pool.kv_heads;
+            it.head = ctl.item_local % a.pool.kv_heads;
+            it.col0 = tile * COLS;
+            it.cols = (int)min((long long)COLS, columns - it.col0);
+            it.first_pos = it.q.len - it.q.n;
+            const int pos_lo = it.first_pos + it.col0 / a.group;
+            it.pos_hi = it.first_pos + (it.col0 + it.cols - 1) / a.group;
+            it.seen_lo = a.window > 0 ? max(0, pos_lo - a.window + 1) : 0;
+            it.k0 = it.seen_lo / KV_TILE * KV_TILE;
+            for (int i = 0; i < 2; ++i) {
+                const int last = min(it.cols, (i + 1) * M_TILE) - 1;  // the M tile's last column
+                const int pos = it.first_pos + (it.col0 + last) / a.group;
+                it.blocks[i] = last < i * M_TILE || pos < it.k0 ? 0 : (pos - it.k0) / BLOCK + 1;
+            }
+            it.most = max(it.blocks[0], it.blocks[1]);
+        }
+        // ---- queries ----
+        if (warp < SOFT_WARPS) {
+            constexpr int EACH = HD / 32;  // consecutive dimensions of a lane
+            for (int c4 = 0; c4 < 32; c4 += 4) {
+                float v[4][EACH];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int c = warp * 32 + c4 + k;
+                    const bool on = c < it.cols;
+                    const int64_t row = it.q.row0 + (on ? (it.col0 + c) / a.group : 0);
+                    const int qh = it.head * a.group + (on ? (it.col0 + c) % a.group : 0);
+                    const int64_t src = row * a.q_stride + (int64_t)qh * HD + lane * EACH;
+#pragma unroll
+                    for (int i = 0; i < EACH; i += 2) {
+                        float2 x = make_float2(0.0f, 0.0f);
+                        if (on) {
+                            if (a.q_type == QMM_OUT_F32) {
+                                x = *reinterpret_cast<const float2*>(static_cast<const float*>(a.q) + src + i);
+                            } else {
+                                x = __bfloat1622float2(
+                                    *reinterpret_cast<const __nv_bfloat162*>(static_cast<const __nv_bfloat16*>(a.q) + src + i));
+                            }
+                        }
+                        v[k][i] = x.x, v[k][i + 1] = x.y;
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int c = warp * 32 + c4 + k;
+                    uint32_t bits = 0;
+#pragma unroll
+                    for (int i = 0; i < EACH; ++i) {
+                        bits = max(bits, __float_as_uint(v[k][i]) & 0x7FFFFFFFu);
+                    }
+                    bits = __reduce_max_sync(0xFFFFFFFFu, bits);
+                    const int exponent = (int)(bits >> 23) - 127;
+                    const int e = bits == 0 || exponent == 128 ? 0 : max(-112, min(120, 12 - exponent));
+                    const float up = __uint_as_float((uint32_t)(e + 127) << 23 | (a.scale < 0.0f ? 0x80000000u : 0u));
+                    uint8_t* row = q_smem + (c / M_TILE) * Shape::Q_BYTES + (c % M_TILE) * 128;
+#pragma unroll
+                    for (int i = 0; i < EACH; i += 2) {
+                        const int dim = lane * EACH + i, chunk = (dim % 64) / 8;
+                        *reinterpret_cast<__half2*>(row + dim / 64 * (M_TILE * 128) + ((chunk ^ (c & 7)) << 4) + dim % 8 * 2) =
+                            __floats2half2_rn(v[k][i] * up, v[k][i + 1] * up);
+                    }
+                    if (lane == 0) {
+                        ctl.q_scale[c] = fabsf(a.scale) * 1.44269504088896340736f * __uint_as_float((uint32_t)(127 - e) << 23);
+                    }
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        __syncthreads();
+
+        if (mma_warp) {
+            // ---- MMAs ----
+            const uint32_t id_s = idesc_f16(BLOCK), id_o = idesc_f16(HD);
+            const uint64_t q_desc = umma_smem_desc(g_smem_u32(q_smem)), k_desc = umma_smem_desc(g_smem_u32(k_smem)),
+                           v_desc = umma_smem_desc(g_smem_u32(v_smem));
+            bool ok = true;
+            auto wait = [&](uint64_t* bar, uint32_t parity) {
+                ok = ok && g_mbar_wait_warp(bar, parity);
+            };
+            auto scores = [&](int i, int kb) {
+                const uint32_t stage = (blocks_before + kb) & 1;
+                fence_after();
+                if (elect_one()) {
+#pragma unroll
+                    for (int kk = 0; kk < HD / 16; ++kk) {
+                        const uint64_t at = 2 * (kk & 3);
+                        umma_ss(tmem + i * BLOCK, q_desc + (uint64_t)((i * Shape::Q_BYTES + (kk >> 2) * M_TILE * 128) >> 4) + at,
+                                k_desc + (uint64_t)((stage * Shape::K_BYTES + (kk >> 2) * BLOCK * 128) >> 4) + at, id_s, kk > 0);
+                    }
+                    umma_commit(&ctl.s_full[i]);
+                }
+                __syncwarp();
+            };
+            auto values = [&](int i, int kb) {
+                const uint32_t stage = (blocks_before + kb) & 1;
+                fence_after();
+                if (elect_one()) {
+#pragma unroll
+                    for (int kk = 0; kk < BLOCK / 16; ++kk) {
+                        umma_ts(tmem + 2 * BLOCK + i * M_TILE, tmem + i * BLOCK + 8 * kk,
+                                v_desc + (uint64_t)((stage * Shape::V_BYTES + (kk >> 2) * HD * 128) >> 4) + 2 * (kk & 3), id_o,
+                                kb > 0 || kk > 0);
+                    }
+                }
+                __syncwarp();
+            };
+            auto commit = [&](uint64_t* bar) {
+                if (elect_one()) {
+                    umma_commit(bar);
+                }
+                __syncwarp();
+            };
+            if (it.most > 0) {
+                wait(&ctl.k_full[blocks_before & 1], blocks_before >> 1 & 1);
+                for (int i = 0; i < 2 && ok; ++i) {
+                    if (it.blocks[i] > 0) {
+                        scores(i, 0);
+                    }
+                }
+                commit(&ctl.k_empty[blocks_before & 1]);
+            }
+            for (int kb = 0; kb < it.most && ok; ++kb) {
+                const uint32_t b = blocks_before + kb;
+                wait(&ctl.v_full[b & 1], b >> 1 & 1);
+                if (kb + 1 < it.most) {
+                    wait(&ctl.k_full[(b + 1) & 1], (b + 1) >> 1 & 1);
+                }
+                for (int i = 0; i < 2 && ok; ++i) {
+                    if (kb < it.blocks[i]) {
+                        wait(&ctl.p_full[i], (tile_before[i] + kb) & 1);
+                        if (ok) {
+                            values(i, kb);
+                        }
+                    }
+                    if (kb + 1 < it.blocks[i] && ok) {
+                        scores(i, kb + 1);
+                    }
+                }
+                commit(&ctl.v_empty[b & 1]);
+                if (kb + 1 < it.most) {
+                    commit(&ctl.k_empty[(b + 1) & 1]);
+                }
+            }
+            commit(&ctl.o_full);
+            if (!ok && lane == 0) {
+                give_up();
+            }
+        } else if (warp >= SOFT_WARPS) {
+            // ---- keys and values ----
+            const int w = warp - SOFT_WARPS, g = lane >> 2, t = lane & 3;
+            bool ok = true;
+            for (int kb = 0; kb < it.most && ok; ++kb) {
+                const uint32_t b = blocks_before + kb, stage = b & 1;
+                const int tok0 = it.k0 + kb * BLOCK + w * KV_TILE;
+                const uint8_t* tile = nullptr;
+                if (tok0 <= it.pos_hi) {
+                    const int page = kv_page(a.pool, a.seqs, it.seq, tok0);
+                    if (page >= 0) {
+                        tile = a.pool.base + kv_tile_index(a.pool, page, it.head, tok0) * TILE;
+                    } else if (lane == 0) {
+                        atomicExch(a.seqs.status, KV_BAD_PAGE);
+                    }
+                }
+                uint32_t kw[2][LANE / 4] = {}, vw[2][LANE / 4] = {}, ks[2][QUANT ? NB : 1] = {}, vs[2][QUANT ? NB : 1] = {};
+                if (tile) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                        for (int i = 0; i < LANE / VEC; ++i) {
+                            load_words<VEC>(kw[j] + i * VEC / 4, tile + j * 32 * LANE + i * 32 * VEC + lane * VEC);
+                            load_words<VEC>(vw[j] + i * VEC / 4, tile + PLANE + SCALES + j * 32 * LANE + i * 32 * VEC + lane * VEC);
+                        }
+                        if (QUANT) {
+                            load_words<(NB >= 4 ? 16 : 8)>(ks[j], tile + PLANE + ((g >> 1) * 2 + j) * NB * 4);
+                            load_words<(NB >= 4 ? 16 : 8)>(vs[j], tile + 2 * PLANE + SCALES + (t * 2 + j) * NB * 4);
+                        }
+                    }
+                }
+                if (b >= 2) {
+                    ok = g_mbar_wait_warp(&ctl.k_empty[stage], ((b >> 1) - 1) & 1);
+                }
+                if (ok) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int key = w * KV_TILE + 8 * j + g;
+#pragma unroll
+                        for (int n = 0; n < NB; ++n) {
+                            uint32_t x[4];
+                            quants<FMT>(kw[j] + n * (U / 4), x);
+                            if (QUANT) {
+                                const __half2 both = as_h2(ks[j][n % (QUANT ? NB : 1)]);
+                                const __half2 d = g & 1 ? __high2half2(both) : __low2half2(both);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    x[i] = h2_bits(__hmul2(as_h2(x[i]), d));
+                                }
+                            }
+                            const int chunk = 4 * (n & 1) + t;  // dimensions 32 n + 8 t .. of the key's row
+                            *reinterpret_cast<uint4*>(k_smem + stage * Shape::K_BYTES + (n >> 1) * BLOCK * 128 + key * 128 +
+                                                      ((chunk ^ (key & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
+                        }
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) {
+                        g_mbar_arrive(&ctl.k_full[stage]);
+                    }
+                    if (b >= 2) {
+                        ok = g_mbar_wait_warp(&ctl.v_empty[stage], ((b >> 1) - 1) & 1);
+                    }
+                }
+                if (ok) {
+                    // tokens that no column sees, and values that are not finite, enter as 0
+                    uint32_t keep[2] = {0xFFFFFFFFu, 0xFFFFFFFFu}, odd[2];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        __half2 sum = as_h2(0u);
+#pragma unroll
+                        for (int n = 0; n < (QUANT ? NB : LANE / 4); ++n) {  // 0, or NaN behind an infinity or a NaN
+                            sum = __hfma2(as_h2(QUANT ? vs[j][n % (QUANT ? NB : 1)] : vw[j][n % (LANE / 4)]), as_h2(0u), sum);
+                        }
+                        odd[j] = h2_bits(sum) & 0x7FFF7FFFu;
+                    }
+                    uint32_t poison = 0;
+                    const bool edge = tok0 < it.seen_lo || tok0 + KV_TILE - 1 > it.pos_hi;
+                    if (__any_sync(0xFFFFFFFFu, (odd[0] | odd[1]) != 0) || edge) {
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const int pos = tok0 + 8 * j + 2 * t + e;
+                                const uint32_t half = e ? 0xFFFF0000u : 0x0000FFFFu;
+                                const bool seen = pos >= it.seen_lo && pos <= it.pos_hi;
+                                // the token's bit of every lane that has some of its dimensions
+                                unsigned int who = __ballot_sync(0xFFFFFFFFu, seen && (odd[j] & half) != 0);
+                                who |= who >> 16;
+                                who |= who >> 8;
+                                who |= who >> 4;
+#pragma unroll
+                                for (int tt = 0; tt < 4; ++tt) {
+                                    poison |= (who >> tt & 1u) << (8 * j + 2 * tt + e);
+                                }
+                                if (!seen || (who >> t & 1u)) {
+                                    keep[j] &= ~half;
+                                }
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int key = w * KV_TILE + 8 * j + 2 * t;
+#pragma unroll
+                        for (int n = 0; n < NB; ++n) {
+                            uint32_t x[4];
+                            quants<FMT>(vw[j] + n * (U / 4), x);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                if (QUANT) {
+                                    x[i] = h2_bits(__hmul2(as_h2(x[i]), as_h2(vs[j][n % (QUANT ? NB : 1)])));
+                                }
+                                // dimension 32 n + 4 g + i is row 32 n + 8 i + g: the lanes' rows differ in their low bits
+                                const int row = 32 * n + 8 * i + g, chunk = key % 64 / 8;
+                                *reinterpret_cast<uint32_t*>(v_smem + stage * Shape::V_BYTES + key / 64 * HD * 128 + row * 128 +
+                                                             ((chunk ^ g) << 4) + key % 8 * 2) = x[i] & keep[j];
+                            }
+                        }
+                    }
+                    if (lane == 0) {
+                        ctl.poison[stage][w] = poison;
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) {
+                        g_mbar_arrive(&ctl.v_full[stage]);
+                    }
+                }
+                if (!ok && lane == 0) {
+                    give_up();
+                }
+            }
+        } else {
+            // ---- softmax: one thread per column ----
+            const int i = warp >> 2, c = threadIdx.x;  // M tile, column of the CTA
+            const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+            const uint32_t s_at = tmem + lanes + i * BLOCK, o_at = tmem + lanes + 2 * BLOCK + i * M_TILE;
+            const float qs = ctl.q_scale[c];
+            const int pos = it.first_pos + (it.col0 + c) / a.group;
+            const int low = a.window > 0 ? pos - a.window + 1 : 0;
+            float m = -INFINITY, l = 0.0f;
+            bool ok = true, poisoned = false;
+            for (int kb = 0; kb < it.blocks[i] && ok; ++kb) {
+                const int key0 = it.k0 + kb * BLOCK;
+                ok = g_mbar_wait_warp(&ctl.s_full[i], (tile_before[i] + kb) & 1);
+                if (!ok) {
+                    break;
+                }
+                fence_after();
+                // keys key0 + lo .. key0 + hi of the block are this column's
+                const int hi = pos - key0, lo = low - key0;
+                const bool whole = __all_sync(0xFFFFFFFFu, hi >= BLOCK - 1 && lo <= 0);
+                float top = -INFINITY;
+                float s[32];
+#pragma unroll
+                for (int part = 0; part < BLOCK / 32; ++part) {
+                    tmem_ld32(s_at + 32 * part, s);
+                    if (!whole) {
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) {
+                            s[k] = 32 * part + k <= hi && 32 * part + k >= lo ? s[k] : -INFINITY;
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) {
+                        top = fmaxf(top, s[k]);
+                    }
+                }
+                top = top == -INFINITY ? top : top * qs;
+                const bool higher = top > m + SLACK || (m == -INFINITY && top > m);
+                if (__any_sync(0xFFFFFFFFu, higher)) {
+                    const float down = higher ? exp2_fast(m - top) : 1.0f;
+                    m = higher ? top : m;
+                    l *= down;
+                    if (kb > 0) {
+#pragma unroll
+                        for (int part = 0; part < HD / 32; ++part) {
+                            tmem_ld32(o_at + 32 * part, s);
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) {
+                                s[k] *= down;
+                            }
+                            tmem_st32(o_at + 32 * part, s);
+                        }
+                        tmem_wait_st();
+                    }
+                }
+                const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+                for (int part = 0; part < BLOCK / 32; ++part) {
+                    uint32_t p[16];
+                    tmem_ld32(s_at + 32 * part, s);
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) {
+                        s[k] = exp2_fast(fmaf(s[k], qs, -ref));
+                        if (!whole) {
+                            s[k] = 32 * part + k <= hi && 32 * part + k >= lo ? s[k] : 0.0f;
+                        }
+                    }
+                    float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        sum0 += s[2 * k];
+                        sum1 += s[2 * k + 1];
+                        p[k] = h2_bits(__floats2half2_rn(s[2 * k], s[2 * k + 1]));
+                    }
+                    l += sum0 + sum1;
+                    tmem_st16(s_at + 16 * part, p);  // over columns that have been read
+                }
+                tmem_wait_st();
+                // a value that is not finite: its stage is filled before the product that this column's arrival allows
+                const uint32_t b = blocks_before + kb;
+                ok = g_mbar_wait_warp(&ctl.v_full[b & 1], b >> 1 & 1);
+                for (int w = 0; w < KV_WARPS; ++w) {
+                    const uint32_t bits = *reinterpret_cast<volatile uint32_t*>(&ctl.poison[b & 1][w]);
+                    for (int k = 0; bits != 0 && k < KV_TILE; ++k) {
+                        const int key = w * KV_TILE + k;
+                        poisoned |= (bits >> k & 1u) && key <= hi && key >= lo;
+                    }
+                }
+                fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    g_mbar_arrive(&ctl.p_full[i]);
+                }
+            }
+            // ---- results ----
+            ok = ok && g_mbar_wait_warp(&ctl.o_full, items_before & 1);
+            if (!ok && lane == 0) {
+                give_up();
+            }
+            fence_after();
+            const int64_t row = it.q.row0 + (it.col0 + c) / a.group;
+            const int qh = it.head * a.group + (it.col0 + c) % a.group;
+            __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + row * a.out_stride + (int64_t)qh * HD;
+            const bool none = it.blocks[i] == 0 || (m == -INFINITY && l == 0.0f);
+            const float inv = none ? 0.0f : poisoned ? __uint_as_float(0x7FC00000u) : 1.0f / l;
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                float o[32];
+                if (it.blocks[i] > 0) {
+                    tmem_ld32(o_at + 32 * n, o);
+                }
+                if (c < it.cols && ok) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {  // dimensions 32 n + 8 k ..: 4 g + j is column 8 j + g
+                        uint32_t x[4];
+#pragma unroll
+                        for (int h = 0; h < 4; ++h) {
+                            const int d = 8 * k + 2 * h, from = 8 * (d & 3) + (d >> 2);
+                            const float x0 = none ? 0.0f : o[from] * inv, x1 = none ? 0.0f : o[from + 8] * inv;
+                            const __nv_bfloat162 pair = __floats2bfloat162_rn(x0, x1);
+                            x[h] = *reinterpret_cast<const uint32_t*>(&pair);
+                        }
+                        *reinterpret_cast<uint4*>(out + 32 * n + 8 * k) = make_uint4(x[0], x[1], x[2], x[3]);
+                    }
+                }
+            }
+            fence_before();
+        }
+        blocks_before += it.most;
+        tile_before[0] += it.blocks[0];
+        tile_before[1] += it.blocks[1];
+        ++items_before;
+        __syncthreads();
+        fence_after();
+    }
+
+    fence_before();
+    __syncthreads();
+    if (mma_warp) {
+        fence_after();
+        __syncwarp();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+        // the last CTA leaves the counters zeroed for the next call
+        if (lane == 0 && atomicAdd(done_ctas, 1u) == gridDim.x - 1) {
+            atomicExch(next_item, 0u);
+            atomicExch(done_ctas, 0u);
+        }
+    }
+}
+
+template <int FMT, int HD>
+cudaError_t launch_prompt(const KvAttnArgs& a, int sm_count, cudaStream_t stream)
+{
+    using Shape = PromptShape<FMT, HD>;
+    auto kernel = kv_prompt_kernel<FMT, HD>;
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) {
+        return e;
+    }
+    static bool configured[64] = {};
+    if (device < 0 || device >= 64 || !configured[device]) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::SMEM);
+        if (e != cudaSuccess) {
+            return e;
+        }
+        if (device >= 0 && device < 64) {
+            configured[device] = true;
+        }
+    }
+    // no more CTAs than there can be items
+    const int64_t items = (a.seqs.rows * a.group / COLS + a.seqs.batch) * a.pool.kv_heads;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>(sm_count, items)));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = Shape::SMEM;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
+template <int FMT>
+cudaError_t launch_prompt_fmt(const KvAttnArgs& a, int sm_count, cudaStream_t stream)
+{
+    return a.pool.head_dim == 64 ? launch_prompt<FMT, 64>(a, sm_count, stream) : launch_prompt<FMT, 128>(a, sm_count, stream);
+}
+
+}  // namespace
+
+// bf16 results of sequences that fill half an M tile on average.
+bool kv_takes_prompt(const KvAttnArgs& a)
+{
+    return a.out_type == QMM_OUT_BF16 && (a.pool.head_dim == 64 || a.pool.head_dim == 128) && a.seqs.row_begin != nullptr &&
+           a.seqs.rows * a.group >= (int64_t)64 * a.seqs.batch;
+}
+
+cudaError_t launch_kv_prompt(const KvAttnArgs& a, int sm_count, cudaStream_t stream)
+{
+    switch (a.pool.fmt) {
+    case FMT_Q4_0: return launch_prompt_fmt<FMT_Q4_0>(a, sm_count, stream);
+    case FMT_Q8_0: return launch_prompt_fmt<FMT_Q8_0>(a, sm_count, stream);
+    default: return launch_prompt_fmt<KV_F16>(a, sm_count, stream);
+    }
+}
+
+}  // namespace qmm

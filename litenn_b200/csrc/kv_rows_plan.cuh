@@ -1,4 +1,5 @@
-// How kv_rows.cu cuts its work: one list of tiles over all (sequence, kv head, pass of eight columns), equal shares of it per CTA.
+// How kv_rows.cu cuts its work: one list over all (sequence, kv head, pass of columns), equal shares of it per CTA.  A list entry
+// has a unit for every tile of 16 tokens, behind KV_ENTRY_UNITS for what an entry costs beside its tiles.
 // Host code too, so that the tests walk it without a GPU.
 #pragma once
 
@@ -6,7 +7,8 @@
 
 namespace qmm {
 
-constexpr int KV_COLS = 8;  // columns (query heads of a kv head, times rows) of a pass
+// Starting an entry (queries, page numbers, the first copies) and joining its warps takes a CTA about as long as this many tiles.
+constexpr int KV_ENTRY_UNITS = 8;
 
 __host__ __device__ __forceinline__ int kv_max(int a, int b)
 {
@@ -16,14 +18,25 @@ __host__ __device__ __forceinline__ int kv_min(int a, int b)
 {
     return a < b ? a : b;
 }
+// Division of numbers below 2^63, in 32 bits where they fit (a 64-bit division is a hundred dependent instructions, and a short
+// call waits for half a dozen of them).
+__host__ __device__ __forceinline__ long long kv_div(long long x, long long y)
+{
+    if (((unsigned long long)(x | y) >> 32) == 0) {
+        return (unsigned int)x / (unsigned int)y;
+    }
+    return x / y;
+}
 
-// A sequence's part of the list: w = kv heads * passes * tiles entries.
+// A sequence's part of the list: kv heads * passes entries.
 struct SeqWork {
     KvSeq q;
     int tile0, tiles, passes;
-    long long w;
+    long long units;
 };
-__host__ __device__ __forceinline__ SeqWork seq_work(const KvPool& c, const KvSeqs& b, int group, int window, int s, bool& bad)
+// `cols` columns (query heads of a kv head, times rows) to a pass.
+__host__ __device__ __forceinline__ SeqWork seq_work(const KvPool& c, const KvSeqs& b, int group, int window, int cols, int s,
+                                                     bool& bad)
 {
     SeqWork x;
     x.q = kv_seq(c, b, s, bad);
@@ -33,8 +46,8 @@ __host__ __device__ __forceinline__ SeqWork seq_work(const KvPool& c, const KvSe
     const int low = window > 0 ? kv_max(0, first - window + 1) : 0;
     x.tile0 = low / KV_TILE;
     x.tiles = kv_max(1, (x.q.len + KV_TILE - 1) / KV_TILE - x.tile0);
-    x.passes = (int)(((long long)x.q.n * group + KV_COLS - 1) / KV_COLS);
-    x.w = (long long)c.kv_heads * x.passes * x.tiles;
+    x.passes = (int)(((long long)x.q.n * group + cols - 1) / cols);
+    x.units = (long long)c.kv_heads * x.passes * (x.tiles + KV_ENTRY_UNITS);
     return x;
 }
 
@@ -45,13 +58,13 @@ struct PassView {
     int seen_lo, all_lo;  // some column sees seen_lo .. pos_hi, every column all_lo .. pos_lo
     int tile_begin, tile_end;  // of the given tiles, those that some column sees
 };
-__host__ __device__ __forceinline__ PassView pass_view(const SeqWork& x, int group, int window, int pass, int tile_begin,
+__host__ __device__ __forceinline__ PassView pass_view(const SeqWork& x, int group, int window, int cols, int pass, int tile_begin,
                                                        int tile_end)
 {
     PassView v;
     const long long columns = (long long)x.q.n * group;
-    v.col0 = pass * KV_COLS;
-    v.cols = columns - v.col0 < KV_COLS ? (int)(columns - v.col0) : KV_COLS;
+    v.col0 = pass * cols;
+    v.cols = columns - v.col0 < cols ? (int)(columns - v.col0) : cols;
     const int first = x.q.len - x.q.n;
     v.pos_lo = first + v.col0 / group;
     v.pos_hi = first + (v.col0 + v.cols - 1) / group;
@@ -62,14 +75,23 @@ __host__ __device__ __forceinline__ PassView pass_view(const SeqWork& x, int gro
     return v;
 }
 
-// `ctas` equal shares of `total` list entries: where share i begins, and which share has an entry.
-__host__ __device__ __forceinline__ long long share_begin(long long total, long long ctas, long long i)
+// CTAs that take a share: one for every eight tiles (a CTA has four warps, which take two at a time), and one for every entry of
+// a short list.
+__host__ __device__ __forceinline__ long long share_count(long long units, long long entries, long long grid)
 {
-    return total * i / ctas;
+    const long long tiles = units - entries * KV_ENTRY_UNITS, want = entries > tiles / 8 ? entries : tiles / 8;
+    return want < grid ? want : grid;
 }
-__host__ __device__ __forceinline__ long long share_of(long long total, long long ctas, long long entry)
+// `ctas` equal shares of `units`, the first ones a unit longer: where share i begins, and which share has a unit.
+__host__ __device__ __forceinline__ long long share_begin(long long units, long long ctas, long long i)
 {
-    return ((entry + 1) * ctas - 1) / total;
+    const long long each = kv_div(units, ctas), more = units - each * ctas;
+    return i * each + (i < more ? i : more);
+}
+__host__ __device__ __forceinline__ long long share_of(long long units, long long ctas, long long unit)
+{
+    const long long each = kv_div(units, ctas), more = units - each * ctas, longer = more * (each + 1);
+    return unit < longer ? kv_div(unit, each + 1) : more + kv_div(unit - longer, each);
 }
 
 }  // namespace qmm

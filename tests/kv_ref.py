@@ -119,3 +119,11 @@ def attention_bound(q, keys, values, scale, bf16_out, half_operands=False):
         ds += dots * 2 * 2.0 ** -11
         rest += 2 * 2.0 ** -11
     return size * (2 * ds + rest + (2.0 ** -8 if bf16_out else 0.0))
+
+
+def norm_bound(hd, q_size, k_size, half_operands):
+    """2-norm of the error over the result's, for independent roundings: bf16's result is off by at most 2^-8 of itself; with
+    fp16 operands each of hd products of a score is off by 2^-11 of itself twice, hd^(1/2) of that in their sum, and
+    probabilities and values by 2^-11 each.  Twice the sum: an upper bound with room for the maxima."""
+    score = 2 * 2.0 ** -11 * q_size * k_size * hd ** 0.5 * hd ** -0.5
+    return 2.0 ** -8 + 2 * (score + 2 * 2.0 ** -11 if half_operands else 2.0 ** -19)

@@ -35,29 +35,34 @@ extern "C" int kv_places(int fmt, int hd)
     return 0;
 }
 
-// Walks the list as the CTAs do.  out[row * kv_heads * group ...]: how often each (row, head, token) is visited, `tokens` per
-// row; returns 0, or what went wrong.
+// Walks the list as the CTAs do, with `cols` columns to a pass.  visits[row][kv head][head of the group][token]: how often each is
+// visited, `tokens` per row; returns 0, or what went wrong.
 extern "C" int kv_walk(int fmt, int kv_heads, int hd, int page_tokens, long long n_pages, int batch, int table_width,
-                       const int* table, const int* kv_len, const int* row_begin, long long rows, int group, int window, int grid,
-                       int tokens, int* visits, int* bad_rows, int* bad_pages)
+                       const int* table, const int* kv_len, const int* row_begin, long long rows, int group, int window, int cols,
+                       int grid, int tokens, int* visits, int* bad_rows, int* bad_pages)
 {
     const KvPool pool = {nullptr, fmt, kv_heads, hd, page_tokens, n_pages};
     const KvSeqs seqs = {batch, table_width, table, kv_len, row_begin, rows, nullptr};
     const long long pool_tiles = n_pages * kv_heads * (page_tokens / KV_TILE);
-    long long total = 0;
+    long long units = 0, entries = 0;
     for (int s = 0; s < batch; ++s) {
         bool bad;
-        total += seq_work(pool, seqs, group, window, s, bad).w;
+        const SeqWork x = seq_work(pool, seqs, group, window, cols, s, bad);
+        units += x.units;
+        entries += (long long)kv_heads * x.passes;
         *bad_rows += bad;
     }
-    if (total == 0) {
+    if (units == 0) {
         return 0;
     }
-    const long long ctas = total / 8 < 1 ? 1 : total / 8 < grid ? total / 8 : grid;
+    const long long ctas = share_count(units, entries, grid);
+    if (ctas < 1 || ctas > grid) {
+        return 14;
+    }
     long long next = 0;
-    std::vector<int> parts(ctas, 0), wanted(ctas, 0);
+    std::vector<int> parts(ctas, 0), wanted(ctas, 0), slots(2 * ctas, 0);
     for (long long c = 0; c < ctas; ++c) {
-        const long long begin = share_begin(total, ctas, c), end = share_begin(total, ctas, c + 1);
+        const long long begin = share_begin(units, ctas, c), end = share_begin(units, ctas, c + 1);
         if (begin != next || end <= begin) {
             return 1;
         }
@@ -65,23 +70,32 @@ extern "C" int kv_walk(int fmt, int kv_heads, int hd, int page_tokens, long long
         int seq = 0;
         long long first = 0;
         bool bad;
-        SeqWork x = seq_work(pool, seqs, group, window, 0, bad);
+        SeqWork x = seq_work(pool, seqs, group, window, cols, 0, bad);
         for (long long at = begin; at < end;) {
-            while (at >= first + x.w) {
-                first += x.w;
+            while (at >= first + x.units) {
+                first += x.units;
                 if (++seq >= batch) {
                     return 2;
                 }
-                x = seq_work(pool, seqs, group, window, seq, bad);
+                x = seq_work(pool, seqs, group, window, cols, seq, bad);
             }
-            const long long entry = (at - first) / x.tiles, e0 = first + entry * x.tiles, e1 = e0 + x.tiles;
+            const int each = x.tiles + KV_ENTRY_UNITS;
+            const long long entry = kv_div(at - first, each);
+            const long long e0 = first + entry * each + KV_ENTRY_UNITS, e1 = e0 + x.tiles;
             const int head = (int)(entry / x.passes), pass = (int)(entry % x.passes);
-            const long long stop = end < e1 ? end : e1;
+            const long long from = at > e0 ? at : e0, to = end < e1 ? end : e1;
+            at = to;
+            if (end < e1) {
+                at = end;
+            }
+            if (from >= to) {
+                continue;
+            }
             if (head >= kv_heads) {
                 return 3;
             }
-            const PassView v = pass_view(x, group, window, pass, x.tile0 + (int)(at - e0), x.tile0 + (int)(stop - e0));
-            if (v.cols < 1 || v.col0 + v.cols > (long long)x.q.n * group) {
+            const PassView v = pass_view(x, group, window, cols, pass, x.tile0 + (int)(from - e0), x.tile0 + (int)(to - e0));
+            if (v.cols < 1 || v.cols > cols || v.col0 + v.cols > (long long)x.q.n * group) {
                 return 4;
             }
             for (int tile = v.tile_begin; tile < v.tile_end; ++tile) {
@@ -117,19 +131,21 @@ extern "C" int kv_walk(int fmt, int kv_heads, int hd, int page_tokens, long long
                     }
                 }
             }
-            const long long c0 = share_of(total, ctas, e0), c1 = share_of(total, ctas, e1 - 1);
-            if (c < c0 || c > c1 || share_begin(total, ctas, c0) > e0 || share_begin(total, ctas, c0 + 1) <= e0) {
+            const long long c0 = share_of(units, ctas, e0), c1 = share_of(units, ctas, e1 - 1);
+            if (c < c0 || c > c1 || share_begin(units, ctas, c0) > e0 || share_begin(units, ctas, c0 + 1) <= e0) {
                 return 10;
+            }
+            if (((from == e0) != (c == c0)) || ((e1 <= end) != (c == c1))) {
+                return 11;
             }
             if (c0 != c1) {
                 ++parts[c0];
                 wanted[c0] = (int)(c1 - c0 + 1);
+                if (slots[2 * c + (from == e0 ? 1 : 0)]++) {
+                    return 15;  // a place of the workspace for two parts
+                }
             }
-            if ((e0 >= begin && e1 <= end) != (c0 == c1)) {
-                return 11;
-            }
-            at = stop;
         }
     }
-    return next != total ? 12 : parts != wanted ? 13 : 0;
+    return next != units ? 12 : parts != wanted ? 13 : 0;
 }

@@ -487,6 +487,132 @@ def test_pool_past_32_bits():
     assert np.abs(np_of(out).reshape(1, kv, hd) - want).max() <= ref.attention_bound(q, kk, vv, hd ** -0.5, False)
 
 
+# ---- prompts: the tensor cores' 128-column tiles -----------------------------------------------------------------------------
+
+def check_prompt(p, rows, lens, heads, rng, bf16=False, window=0, q_scale=2.0, poison=()):
+    """bf16 results against 64 bits, element by element and in the 2-norm."""
+    ks, vs = p.fill(rng)
+    q = (rng.standard_normal((sum(rows), heads, p.hd)) * q_scale).astype(np.float32)
+    if bf16:
+        q = ref.bf16_round(q)
+    got = p.attend(q, rows, lens, heads, bf16, True, window)
+    at, off, size = 0, 0.0, 0.0
+    for s, (n, r) in enumerate(zip(lens, rows)):
+        if r == 0:
+            continue
+        want = ref.attention(q[at:at + r], ks[s], vs[s], n, p.hd ** -0.5, window)
+        err = np.abs(got[at:at + r] - want)
+        assert err.max() <= ref.attention_bound(q[at:at + r], ks[s], vs[s], p.hd ** -0.5, True, True), (s, err.max())
+        off, size = off + (err ** 2).sum(), size + (want ** 2).sum()
+        at += r
+    assert off <= size * ref.norm_bound(p.hd, q_scale, 1.0, True) ** 2, (off / size) ** 0.5
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("hd,heads,kv_heads,page", [(128, 2, 2, 64), (64, 8, 2, 16), (128, 7, 1, 32)])
+@pytest.mark.parametrize("rows,lens", [([256], [256]), ([130, 1, 0, 67], [130, 40, 9, 300]), ([100], [1000]), ([300], [301])])
+def test_prompts(fmt, hd, heads, kv_heads, page, rows, lens):
+    p = Paged(fmt, kv_heads, hd, page, lens, seed=sum(rows))
+    check_prompt(p, rows, lens, heads, np.random.default_rng(hd + sum(lens)), bf16=heads == 7)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("window", [1, 17, 200])
+def test_prompts_with_windows(fmt, window):
+    p = Paged(fmt, 1, 128, 16, [500, 90])
+    check_prompt(p, [333, 90], [500, 90], 2, np.random.default_rng(window), window=window)
+
+
+def test_prompts_of_more_items_than_sms():
+    lens = [64 + 3 * i for i in range(90)]
+    p = Paged(ref.Q4_0, 2, 64, 16, lens)
+    check_prompt(p, [64] * 90, lens, 4, np.random.default_rng(20))
+
+
+def test_prompts_whose_scores_grow_along_the_keys():
+    """The running maximum moves by more than its slack again and again."""
+    rng = np.random.default_rng(21)
+    n, hd = 700, 128
+    p = Paged(ref.F16, 1, hd, 64, [n])
+    k = rng.standard_normal((n, 1, hd)).astype(np.float32) * np.linspace(0.05, 4, n)[:, None, None].astype(np.float32)
+    v = rng.standard_normal((n, 1, hd)).astype(np.float32)
+    kd, vd = torch_of(k), torch_of(v)
+    p.cache.append(p.batch([n], [n]), None, 0, 0, 0, 0, kd.data_ptr(), hd, vd.data_ptr(), hd, 0, 0, 0)
+    q = rng.standard_normal((128, 2, hd)).astype(np.float32) * 4
+    got = p.attend(q, [128], [n], 2, out_bf16=True)
+    kk, vv = ref.stored(k, ref.F16), ref.stored(v, ref.F16)
+    want = ref.attention(q, kk, vv, n, hd ** -0.5)
+    assert np.linalg.norm(got - want) <= np.linalg.norm(want) * ref.norm_bound(hd, 4.0, 4.0, True)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_prompts_what_a_row_does_not_see_does_not_reach_it(fmt):
+    rng = np.random.default_rng(22)
+    n, rows, hd, heads = 400, 200, 128, 2
+    p = Paged(fmt, 1, hd, 16, [n])
+    k = rng.standard_normal((n, 1, hd)).astype(np.float32)
+    v = rng.standard_normal((n, 1, hd)).astype(np.float32)
+    k[250, 0, 3], v[330, 0, 70], v[20, 0, 1] = np.nan, np.inf, np.nan  # token 20 lies in front of every window
+    kd, vd = torch_of(k), torch_of(v)
+    p.cache.append(p.batch([n], [n]), None, 0, 0, 0, 0, kd.data_ptr(), hd, vd.data_ptr(), hd, 0, 0, 0)
+    q = rng.standard_normal((rows, heads, hd)).astype(np.float32)
+    got = p.attend(q, [rows], [n], heads, out_bf16=True, window=100)
+    pos = np.arange(n - rows, n)
+    sees = ((pos >= 250) & (pos < 350)) | (pos >= 330)
+    assert np.isfinite(got[~sees]).all() and not np.isfinite(got[sees][:, :, 70]).any()
+    kk, vv = np.nan_to_num(ref.stored(k, fmt)), ref.stored(v, fmt)
+    vv = np.where(np.isfinite(vv), vv, 0)
+    want = ref.attention(q, kk, vv, n, hd ** -0.5, 100)[~sees]
+    assert np.linalg.norm(got[~sees] - want) <= np.linalg.norm(want) * ref.norm_bound(hd, 1.0, 1.0, True)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_prompts_rows_that_see_nothing_and_padding(fmt):
+    rng = np.random.default_rng(23)
+    p = Paged(fmt, 1, 64, 16, [30, 0])
+    ks, vs = p.fill(rng)
+    q = rng.standard_normal((250, 2, 64)).astype(np.float32)
+    got = p.attend(q, [130, 70], [30, 0], 2, out_bf16=True, total=250)
+    assert (got[:100] == 0).all() and (got[130:200] == 0).all() and (got[200:] == 7).all()
+    want = ref.attention(q[100:130], ks[0], vs[0], 30, 0.125)
+    assert np.linalg.norm(got[100:130] - want) <= np.linalg.norm(want) * ref.norm_bound(64, 1.0, 1.0, True)
+
+
+def test_prompts_repeat_bit_for_bit_and_leave_the_workspace_clean():
+    rng = np.random.default_rng(24)
+    import torch
+    p = Paged(ref.Q4_0, 4, 64, 16, [600, 200])
+    p.fill(rng)
+    q = rng.standard_normal((700, 8, 64)).astype(np.float32)
+    first = p.attend(q, [500, 200], [600, 200], 8, out_bf16=True)
+    for _ in range(3):
+        np.testing.assert_array_equal(p.attend(q, [500, 200], [600, 200], 8, out_bf16=True), first)
+    assert int(p.workspace[:16384].to(torch.int32).sum()) == 0
+
+
+def test_prompts_bad_pages_and_rows():
+    rng = np.random.default_rng(25)
+    import torch
+    p = Paged(ref.Q4_0, 1, 64, 16, [200, 200])
+    ks, vs = p.fill(rng)
+    good = p.table_dev.clone()
+    q = rng.standard_normal((200, 2, 64)).astype(np.float32)
+    qd, out = torch_of(q.reshape(200, -1)), torch.zeros(200, 128, device="cuda", dtype=torch.bfloat16)
+
+    def attend(b):
+        p.cache.attend(b, 2, qd.data_ptr(), 0, 128, out.data_ptr(), 1, 128, 0.125, 0, p.workspace.data_ptr())
+
+    for page in (-1, p.n_pages):
+        p.table_dev[0, 5] = page
+        assert "21" in status_of(lambda: attend(p.batch([100, 100], [200, 200])))
+        want = ref.attention(q[100:], ks[1], vs[1], 200, 0.125)
+        assert np.linalg.norm(np_of(out)[100:].reshape(100, 2, 64) - want) <= np.linalg.norm(want) * ref.norm_bound(64, 1.0, 1.0, True)
+    p.table_dev.copy_(good)
+    assert "22" in status_of(lambda: attend(p.batch([100, 100], [p.width * 16 + 1, 200])))
+    assert "22" in status_of(lambda: attend(p.batch([100, 150], [200, 200], total=200)))
+    assert int(p.workspace[:16384].to(torch.int32).sum()) == 0
+
+
 # ---- what cannot be right is reported -------------------------------------------------------------------------------------
 
 def status_of(call):

@@ -13,7 +13,7 @@ I32 = np.ctypeslib.ndpointer(dtype=np.int32)
 def lib():
     L = native_build.load("kv_plan", False)
     L.kv_walk.argtypes = [ctypes.c_int] * 4 + [ctypes.c_longlong] + [ctypes.c_int] * 2 + [I32, I32, ctypes.c_void_p,
-                                                                                          ctypes.c_longlong] + [ctypes.c_int] * 4 + \
+                                                                                          ctypes.c_longlong] + [ctypes.c_int] * 5 + \
         [I32, ctypes.POINTER(ctypes.c_int), ctypes.POINTER(ctypes.c_int)]
     return L
 
@@ -24,7 +24,7 @@ def test_every_value_has_a_place_of_its_own(lib, fmt, hd):
     assert lib.kv_places(fmt, hd) == 0
 
 
-def walk(lib, page, rows, lens, group, kv_heads, window, grid, table=None, begin="sums", total=None, n_pages=None, width=None):
+def walk(lib, page, rows, lens, group, kv_heads, window, grid, cols=8, table=None, begin="sums", total=None, n_pages=None, width=None):
     width = width or max(1, max(-(-n // page) for n in lens))
     n_pages = n_pages or len(lens) * width
     if table is None:
@@ -36,7 +36,7 @@ def walk(lib, page, rows, lens, group, kv_heads, window, grid, table=None, begin
     visits = np.zeros((max(total, 1), kv_heads, group, tokens), dtype=np.int32)
     bad_rows, bad_pages = ctypes.c_int(), ctypes.c_int()
     rc = lib.kv_walk(1, kv_heads, 128, page, n_pages, len(lens), width, table, np.asarray(lens, dtype=np.int32),
-                     None if b is None else b.ctypes.data, total, group, window, grid, tokens, visits, bad_rows, bad_pages)
+                     None if b is None else b.ctypes.data, total, group, window, cols, grid, tokens, visits, bad_rows, bad_pages)
     assert rc == 0, rc
     return visits, bad_rows.value, bad_pages.value
 
@@ -45,9 +45,10 @@ def walk(lib, page, rows, lens, group, kv_heads, window, grid, table=None, begin
                                        ([1], [5000]), ([0, 0], [3, 0])])
 @pytest.mark.parametrize("group,kv_heads", [(1, 3), (8, 2), (7, 1), (24, 1)])
 @pytest.mark.parametrize("window", [0, 1, 37])
-@pytest.mark.parametrize("grid", [1, 7, 444])
-def test_every_pair_is_visited_once(lib, rows, lens, group, kv_heads, window, grid):
-    visits, bad_rows, bad_pages = walk(lib, 32, rows, lens, group, kv_heads, window, grid)
+@pytest.mark.parametrize("grid", [1, 7, 592])
+@pytest.mark.parametrize("cols", [8, 16])
+def test_every_pair_is_visited_once(lib, rows, lens, group, kv_heads, window, grid, cols):
+    visits, bad_rows, bad_pages = walk(lib, 32, rows, lens, group, kv_heads, window, grid, cols)
     assert bad_rows == bad_pages == 0
     at = 0
     for r, n in zip(rows, lens):
@@ -80,6 +81,6 @@ def test_rows_and_lengths_that_cannot_be_right_are_left_out(lib, lens, begin):
     visits = np.zeros((2, 1, 2, tokens), dtype=np.int32)
     bad_rows, bad_pages = ctypes.c_int(), ctypes.c_int()
     rc = lib.kv_walk(1, 1, 128, 16, 6, 2, width, np.arange(6, dtype=np.int32), np.array(lens, dtype=np.int32),
-                     np.array(begin, dtype=np.int32).ctypes.data, 2, 2, 0, 444, tokens, visits, bad_rows, bad_pages)
+                     np.array(begin, dtype=np.int32).ctypes.data, 2, 2, 0, 8, 444, tokens, visits, bad_rows, bad_pages)
     assert rc == 0 and bad_rows.value >= 1 and bad_pages.value == 0
     assert visits.max() <= 1 and visits[:, :, :, 40:].sum() == 0
