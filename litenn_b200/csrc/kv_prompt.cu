@@ -15,6 +15,7 @@
 // fp32.  A value that is not finite would reach every column of the product (0 times infinity): it enters as 0, and
 // the columns that see its token are made NaN.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_kernels.h"
 #include "kv_rows_plan.cuh"
@@ -28,7 +29,8 @@ namespace {
 
 constexpr int BLOCK = 128;                     // keys per block
 constexpr int M_TILE = 128, COLS = 2 * M_TILE; // columns of an M tile, of a CTA
-constexpr int SOFT_WARPS = 8, KV_WARPS = 8;
+constexpr int KV_TILES = BLOCK / KV_TILE;       // tiles of a block
+constexpr int SOFT_WARPS = 8, KV_WARPS = KV_TILES;
 constexpr int THREADS = (SOFT_WARPS + KV_WARPS + 1) * 32;
 constexpr uint32_t TMEM_COLS = 512;            // S0, S1, O0, O1
 constexpr int KV_LATE_PROMPT = 24;             // a bounded wait ran out
@@ -44,12 +46,24 @@ struct PromptShape {
     static constexpr int SMEM = 1024 + CONTROL + 2 * Q_BYTES + 2 * K_BYTES + 2 * V_BYTES;
 };
 
+// What a CTA works on: 256 columns of a kv head of a sequence.
+struct Item {
+    KvSeq q;
+    int seq, head;
+    int col0, cols;       // of the sequence's columns
+    int first_pos;        // of row 0
+    int k0;               // first key, a multiple of 16
+    int blocks[2], most;  // of each M tile
+    int pos_hi, seen_lo;  // keys that some column sees
+};
+
 struct Control {
     uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full;
     uint32_t tmem;
+    Item item;
     int item_seq, item_local;
     int late;
-    uint32_t poison[2][KV_WARPS];  // per stage and tile: tokens whose value is not finite
+    uint32_t poison[2][KV_TILES];  // per stage and tile: tokens whose value is not finite
     float q_scale[COLS];
 };
 
@@ -80,38 +94,34 @@ __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint
         "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
         : "memory");
 }
-__device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&r)[32])
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&r)[16])
 {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
-        "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]),
-          "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]), "=f"(r[17]), "=f"(r[18]),
-          "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]),
-          "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
         : "r"(addr)
         : "memory");
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const float (&r)[32])
+// The loads have come; `r` is named so that nothing reads it earlier.
+__device__ __forceinline__ void tmem_wait_ld(float (&r)[16])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]), "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const float (&r)[16])
 {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
-        "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
-        "f"(r[0]), "f"(r[1]), "f"(r[2]), "f"(r[3]), "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7]), "f"(r[8]), "f"(r[9]), "f"(r[10]),
-        "f"(r[11]), "f"(r[12]), "f"(r[13]), "f"(r[14]), "f"(r[15]), "f"(r[16]), "f"(r[17]), "f"(r[18]), "f"(r[19]), "f"(r[20]),
-        "f"(r[21]), "f"(r[22]), "f"(r[23]), "f"(r[24]), "f"(r[25]), "f"(r[26]), "f"(r[27]), "f"(r[28]), "f"(r[29]), "f"(r[30]),
-        "f"(r[31])
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
+        "f"(r[0]), "f"(r[1]), "f"(r[2]), "f"(r[3]), "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7]), "f"(r[8]), "f"(r[9]), "f"(r[10]), "f"(r[11]), "f"(r[12]), "f"(r[13]), "f"(r[14]), "f"(r[15])
         : "memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16])
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8])
 {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(
-            addr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-        : "memory");
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st()
 {
@@ -130,6 +140,14 @@ __device__ __forceinline__ float exp2_fast(float x)
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// Four 8 x 8 matrices of fp16, rows of 16 bytes: lane 4g + t holds row g, columns 2t and 2t + 1 of each, lane 8m + r names the
+// place of row r of matrix m.
+__device__ __forceinline__ void store_matrices(void* row, const uint32_t (&x)[4])
+{
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(g_smem_u32(row)), "r"(x[0]), "r"(x[1]),
+                 "r"(x[2]), "r"(x[3])
+                 : "memory");
 }
 __device__ __forceinline__ uint32_t h2_bits(__half2 h)
 {
@@ -170,23 +188,12 @@ __device__ __forceinline__ void load_words(uint32_t* w, const uint8_t* p)
     }
 }
 
-// What a CTA works on: 256 columns of a kv head of a sequence.
-struct Item {
-    KvSeq q;
-    int seq, head;
-    int col0, cols;       // of the sequence's columns
-    int first_pos;        // of row 0
-    int k0;               // first key, a multiple of 16
-    int blocks[2], most;  // of each M tile
-    int pos_hi, seen_lo;  // keys that some column sees
-};
-
 template <int FMT, int HD>
 __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs a)
 {
     using Shape = PromptShape<FMT, HD>;
     constexpr int NB = HD / 32, TILE = kv_tile_bytes(FMT, HD), PLANE = kv_plane_bytes(FMT, HD), SCALES = kv_scale_bytes(FMT, HD);
-    constexpr int U = kv_unit(FMT), LANE = kv_lane_bytes(FMT, HD), VEC = kv_vec(FMT, HD), VB = VEC / U;
+    constexpr int U = kv_unit(FMT), LANE = kv_lane_bytes(FMT, HD), VEC = kv_vec(FMT, HD);
     constexpr bool QUANT = FMT != KV_F16;
     extern __shared__ uint8_t prompt_smem[];
     uint8_t* smem = prompt_smem + ((1024u - (g_smem_u32(prompt_smem) & 1023u)) & 1023u);
@@ -225,7 +232,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
 
     unsigned int* next_item = reinterpret_cast<unsigned int*>(a.workspace + KV_COUNTER_BYTES);
     unsigned int* done_ctas = next_item + 1;
-    uint32_t blocks_before = 0, tile_before[2] = {0, 0}, items_before = 0;  // completed: the barriers' parities
+    uint32_t blocks_before = 0, before0 = 0, before1 = 0, items_before = 0;  // completed: the barriers' parities
     auto give_up = [&]() {
         atomicExch(a.seqs.status, KV_LATE_PROMPT);
         *reinterpret_cast<volatile int*>(&ctl.late) = 1;
@@ -278,29 +285,33 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
         if (ctl.item_seq < 0 || ctl.late) {
             break;
         }
-        Item it;
-        {
+        const Item& it = ctl.item;
+        if (threadIdx.x == 0) {
+            Item n;
             bool bad;
-            it.seq = ctl.item_seq;
-            it.q = kv_seq(a.pool, a.seqs, it.seq, bad);
-            const long long columns = (long long)it.q.n * a.group;
+            n.seq = ctl.item_seq;
+            n.q = kv_seq(a.pool, a.seqs, n.seq, bad);
+            const long long columns = (long long)n.q.n * a.group;
             const int tiles = (int)((columns + COLS - 1) / COLS);
             const int tile = tiles - 1 - ctl.item_local / a.pool.kv_heads;
-            it.head = ctl.item_local % a.pool.kv_heads;
-            it.col0 = tile * COLS;
-            it.cols = (int)min((long long)COLS, columns - it.col0);
-            it.first_pos = it.q.len - it.q.n;
-            const int pos_lo = it.first_pos + it.col0 / a.group;
-            it.pos_hi = it.first_pos + (it.col0 + it.cols - 1) / a.group;
-            it.seen_lo = a.window > 0 ? max(0, pos_lo - a.window + 1) : 0;
-            it.k0 = it.seen_lo / KV_TILE * KV_TILE;
+            n.head = ctl.item_local % a.pool.kv_heads;
+            n.col0 = tile * COLS;
+            n.cols = (int)min((long long)COLS, columns - n.col0);
+            n.first_pos = n.q.len - n.q.n;
+            const int pos_lo = n.first_pos + n.col0 / a.group;
+            n.pos_hi = n.first_pos + (n.col0 + n.cols - 1) / a.group;
+            n.seen_lo = a.window > 0 ? max(0, pos_lo - a.window + 1) : 0;
+            n.k0 = n.seen_lo / KV_TILE * KV_TILE;
+#pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int last = min(it.cols, (i + 1) * M_TILE) - 1;  // the M tile's last column
-                const int pos = it.first_pos + (it.col0 + last) / a.group;
-                it.blocks[i] = last < i * M_TILE || pos < it.k0 ? 0 : (pos - it.k0) / BLOCK + 1;
+                const int last = min(n.cols, (i + 1) * M_TILE) - 1;  // the M tile's last column
+                const int pos = n.first_pos + (n.col0 + last) / a.group;
+                n.blocks[i] = last < i * M_TILE || pos < n.k0 ? 0 : (pos - n.k0) / BLOCK + 1;
             }
-            it.most = max(it.blocks[0], it.blocks[1]);
+            n.most = max(n.blocks[0], n.blocks[1]);
+            ctl.item = n;
         }
+        __syncthreads();
         // ---- queries ----
         if (warp < SOFT_WARPS) {
             constexpr int EACH = HD / 32;  // consecutive dimensions of a lane
@@ -397,34 +408,38 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
                 }
                 __syncwarp();
             };
-            if (it.most > 0) {
+            const int most = it.most, blocks0 = it.blocks[0], blocks1 = it.blocks[1];
+            if (most > 0) {
                 wait(&ctl.k_full[blocks_before & 1], blocks_before >> 1 & 1);
-                for (int i = 0; i < 2 && ok; ++i) {
-                    if (it.blocks[i] > 0) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    if ((i ? blocks1 : blocks0) > 0 && ok) {
                         scores(i, 0);
                     }
                 }
                 commit(&ctl.k_empty[blocks_before & 1]);
             }
-            for (int kb = 0; kb < it.most && ok; ++kb) {
+            for (int kb = 0; kb < most && ok; ++kb) {
                 const uint32_t b = blocks_before + kb;
                 wait(&ctl.v_full[b & 1], b >> 1 & 1);
-                if (kb + 1 < it.most) {
+                if (kb + 1 < most) {
                     wait(&ctl.k_full[(b + 1) & 1], (b + 1) >> 1 & 1);
                 }
-                for (int i = 0; i < 2 && ok; ++i) {
-                    if (kb < it.blocks[i]) {
-                        wait(&ctl.p_full[i], (tile_before[i] + kb) & 1);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int mine = i ? blocks1 : blocks0;
+                    if (kb < mine && ok) {
+                        wait(&ctl.p_full[i], ((i ? before1 : before0) + kb) & 1);
                         if (ok) {
                             values(i, kb);
                         }
                     }
-                    if (kb + 1 < it.blocks[i] && ok) {
+                    if (kb + 1 < mine && ok) {
                         scores(i, kb + 1);
                     }
                 }
                 commit(&ctl.v_empty[b & 1]);
-                if (kb + 1 < it.most) {
+                if (kb + 1 < most) {
                     commit(&ctl.k_empty[(b + 1) & 1]);
                 }
             }
@@ -436,33 +451,62 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
             // ---- keys and values ----
             const int w = warp - SOFT_WARPS, g = lane >> 2, t = lane & 3;
             bool ok = true;
-            for (int kb = 0; kb < it.most && ok; ++kb) {
-                const uint32_t b = blocks_before + kb, stage = b & 1;
+            const int most = it.most;
+            // lane n holds where this warp's tile of block n (and 32 + n, ...) lies, 0 where there is none
+            auto where = [&](int kb) -> unsigned long long {
                 const int tok0 = it.k0 + kb * BLOCK + w * KV_TILE;
-                const uint8_t* tile = nullptr;
-                if (tok0 <= it.pos_hi) {
-                    const int page = kv_page(a.pool, a.seqs, it.seq, tok0);
-                    if (page >= 0) {
-                        tile = a.pool.base + kv_tile_index(a.pool, page, it.head, tok0) * TILE;
-                    } else if (lane == 0) {
-                        atomicExch(a.seqs.status, KV_BAD_PAGE);
-                    }
+                if (kb >= most || tok0 > it.pos_hi) {
+                    return 0;
                 }
-                uint32_t kw[2][LANE / 4] = {}, vw[2][LANE / 4] = {}, ks[2][QUANT ? NB : 1] = {}, vs[2][QUANT ? NB : 1] = {};
-                if (tile) {
+                const int page = kv_page(a.pool, a.seqs, it.seq, tok0);
+                if (page < 0) {
+                    atomicExch(a.seqs.status, KV_BAD_PAGE);
+                    return 0;
+                }
+                return reinterpret_cast<unsigned long long>(a.pool.base + kv_tile_index(a.pool, page, it.head, tok0) * TILE);
+            };
+            unsigned long long places = most > 0 ? where(lane) : 0;
+            auto place_of = [&](int kb) -> const uint8_t* {
+                return reinterpret_cast<const uint8_t*>(__shfl_sync(0xFFFFFFFFu, places, kb & 31));
+            };
+            // raw words of a tile's keys and of its values: asked for as soon as the ones before have been converted
+            uint32_t kw[2][LANE / 4], vw[2][LANE / 4], ks[2][QUANT ? NB : 1], vs[2][QUANT ? NB : 1];
+            auto ask = [&](uint32_t (&x)[2][LANE / 4], uint32_t (&d)[2][QUANT ? NB : 1], const uint8_t* plane, int scale_at) {
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
+                for (int j = 0; j < 2; ++j) {
+                    if (plane) {
 #pragma unroll
                         for (int i = 0; i < LANE / VEC; ++i) {
-                            load_words<VEC>(kw[j] + i * VEC / 4, tile + j * 32 * LANE + i * 32 * VEC + lane * VEC);
-                            load_words<VEC>(vw[j] + i * VEC / 4, tile + PLANE + SCALES + j * 32 * LANE + i * 32 * VEC + lane * VEC);
+                            load_words<VEC>(x[j] + i * VEC / 4, plane + j * 32 * LANE + i * 32 * VEC + lane * VEC);
                         }
                         if (QUANT) {
-                            load_words<(NB >= 4 ? 16 : 8)>(ks[j], tile + PLANE + ((g >> 1) * 2 + j) * NB * 4);
-                            load_words<(NB >= 4 ? 16 : 8)>(vs[j], tile + 2 * PLANE + SCALES + (t * 2 + j) * NB * 4);
+                            load_words<(NB >= 4 ? 16 : 8)>(d[j], plane + PLANE + (scale_at * 2 + j) * NB * 4);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < LANE / 4; ++i) {
+                            x[j][i] = 0;
+                        }
+#pragma unroll
+                        for (int i = 0; i < (QUANT ? NB : 1); ++i) {
+                            d[j][i] = 0;
                         }
                     }
                 }
+            };
+            const uint8_t* tile = nullptr;
+            if (most > 0) {
+                tile = place_of(0);
+                ask(kw, ks, tile, g >> 1);
+                ask(vw, vs, tile ? tile + PLANE + SCALES : nullptr, t);
+            }
+            for (int kb = 0; kb < most && ok; ++kb) {
+                const uint32_t b = blocks_before + kb, stage = b & 1;
+                const int tok0 = it.k0 + kb * BLOCK + w * KV_TILE;
+                if ((kb & 31) == 31) {
+                    places = where(kb + 1 + lane);
+                }
+                const uint8_t* next = place_of(kb + 1);  // nothing behind the last block
                 if (b >= 2) {
                     ok = g_mbar_wait_warp(&ctl.k_empty[stage], ((b >> 1) - 1) & 1);
                 }
@@ -475,8 +519,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
                             uint32_t x[4];
                             quants<FMT>(kw[j] + n * (U / 4), x);
                             if (QUANT) {
-                                const __half2 both = as_h2(ks[j][n % (QUANT ? NB : 1)]);
-                                const __half2 d = g & 1 ? __high2half2(both) : __low2half2(both);
+                                const uint32_t both = ks[j][n % (QUANT ? NB : 1)];
+                                const __half2 d = as_h2(__byte_perm(both, both, g & 1 ? 0x3232u : 0x1010u));
 #pragma unroll
                                 for (int i = 0; i < 4; ++i) {
                                     x[i] = h2_bits(__hmul2(as_h2(x[i]), d));
@@ -484,7 +528,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
                             }
                             const int chunk = 4 * (n & 1) + t;  // dimensions 32 n + 8 t .. of the key's row
                             *reinterpret_cast<uint4*>(k_smem + stage * Shape::K_BYTES + (n >> 1) * BLOCK * 128 + key * 128 +
-                                                      ((chunk ^ (key & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
+                                                      ((chunk ^ g) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
                         }
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -492,13 +536,14 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
                     if (lane == 0) {
                         g_mbar_arrive(&ctl.k_full[stage]);
                     }
+                    ask(kw, ks, next, g >> 1);
                     if (b >= 2) {
                         ok = g_mbar_wait_warp(&ctl.v_empty[stage], ((b >> 1) - 1) & 1);
                     }
                 }
                 if (ok) {
                     // tokens that no column sees, and values that are not finite, enter as 0
-                    uint32_t keep[2] = {0xFFFFFFFFu, 0xFFFFFFFFu}, odd[2];
+                    uint32_t odd[2];
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         __half2 sum = as_h2(0u);
@@ -510,7 +555,33 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
                     }
                     uint32_t poison = 0;
                     const bool edge = tok0 < it.seen_lo || tok0 + KV_TILE - 1 > it.pos_hi;
+                    auto put = [&](auto masked, const uint32_t (&keep)[2]) {
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                            for (int n = 0; n < NB; ++n) {
+                                uint32_t x[4];
+                                quants<FMT>(vw[j] + n * (U / 4), x);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    if (QUANT) {
+                                        x[i] = h2_bits(__hmul2(as_h2(x[i]), as_h2(vs[j][n % (QUANT ? NB : 1)])));
+                                    }
+                                    if (decltype(masked)::value) {
+                                        x[i] &= keep[j];
+                                    }
+                                }
+                                // dimension 32 n + 4 g + i is row 32 n + 8 i + g: four matrices of 8 rows x 8 tokens.  This
+                                // lane's row for the store is 32 n + lane; its 16 bytes are tokens 8 j .. of the tile
+                                const int chunk = (w * KV_TILE + 8 * j) % 64 / 8;
+                                store_matrices(v_smem + stage * Shape::V_BYTES + w * KV_TILE / 64 * HD * 128 + (32 * n + lane) * 128 +
+                                                   ((chunk ^ (lane & 7)) << 4),
+                                               x);
+                            }
+                        }
+                    };
                     if (__any_sync(0xFFFFFFFFu, (odd[0] | odd[1]) != 0) || edge) {
+                        uint32_t keep[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
 #pragma unroll
@@ -532,25 +603,10 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
                                 }
                             }
                         }
-                    }
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const int key = w * KV_TILE + 8 * j + 2 * t;
-#pragma unroll
-                        for (int n = 0; n < NB; ++n) {
-                            uint32_t x[4];
-                            quants<FMT>(vw[j] + n * (U / 4), x);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                if (QUANT) {
-                                    x[i] = h2_bits(__hmul2(as_h2(x[i]), as_h2(vs[j][n % (QUANT ? NB : 1)])));
-                                }
-                                // dimension 32 n + 4 g + i is row 32 n + 8 i + g: the lanes' rows differ in their low bits
-                                const int row = 32 * n + 8 * i + g, chunk = key % 64 / 8;
-                                *reinterpret_cast<uint32_t*>(v_smem + stage * Shape::V_BYTES + key / 64 * HD * 128 + row * 128 +
-                                                             ((chunk ^ g) << 4) + key % 8 * 2) = x[i] & keep[j];
-                            }
-                        }
+                        put(std::true_type{}, keep);
+                    } else {
+                        const uint32_t all[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
+                        put(std::false_type{}, all);
                     }
                     if (lane == 0) {
                         ctl.poison[stage][w] = poison;
@@ -560,6 +616,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
                     if (lane == 0) {
                         g_mbar_arrive(&ctl.v_full[stage]);
                     }
+                    ask(vw, vs, next ? next + PLANE + SCALES : nullptr, t);
                 }
                 if (!ok && lane == 0) {
                     give_up();
@@ -575,82 +632,105 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
             const int low = a.window > 0 ? pos - a.window + 1 : 0;
             float m = -INFINITY, l = 0.0f;
             bool ok = true, poisoned = false;
-            for (int kb = 0; kb < it.blocks[i] && ok; ++kb) {
+            const int my_blocks = it.blocks[i];
+            const uint32_t my_before = i ? before1 : before0;
+            for (int kb = 0; kb < my_blocks && ok; ++kb) {
                 const int key0 = it.k0 + kb * BLOCK;
-                ok = g_mbar_wait_warp(&ctl.s_full[i], (tile_before[i] + kb) & 1);
+                ok = g_mbar_wait_warp(&ctl.s_full[i], (my_before + kb) & 1);
                 if (!ok) {
                     break;
                 }
                 fence_after();
                 // keys key0 + lo .. key0 + hi of the block are this column's
                 const int hi = pos - key0, lo = low - key0;
-                const bool whole = __all_sync(0xFFFFFFFFu, hi >= BLOCK - 1 && lo <= 0);
-                float top = -INFINITY;
-                float s[32];
+                auto probabilities = [&](auto all_seen) {
+                    constexpr bool WHOLE = decltype(all_seen)::value;
+                    constexpr int PARTS = BLOCK / 16;
+                    float s[2][16];  // the next 16 scores are on their way while these are worked on
+                    float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    tmem_ld16(s_at, s[0]);
+                    tmem_wait_ld(s[0]);
 #pragma unroll
-                for (int part = 0; part < BLOCK / 32; ++part) {
-                    tmem_ld32(s_at + 32 * part, s);
-                    if (!whole) {
+                    for (int part = 0; part < PARTS; ++part) {
+                        float (&x)[16] = s[part & 1];
+                        tmem_ld16(s_at + 16 * ((part + 1) % PARTS), s[(part + 1) & 1]);
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) {
-                            s[k] = 32 * part + k <= hi && 32 * part + k >= lo ? s[k] : -INFINITY;
-                        }
-                    }
-#pragma unroll
-                    for (int k = 0; k < 32; ++k) {
-                        top = fmaxf(top, s[k]);
-                    }
-                }
-                top = top == -INFINITY ? top : top * qs;
-                const bool higher = top > m + SLACK || (m == -INFINITY && top > m);
-                if (__any_sync(0xFFFFFFFFu, higher)) {
-                    const float down = higher ? exp2_fast(m - top) : 1.0f;
-                    m = higher ? top : m;
-                    l *= down;
-                    if (kb > 0) {
-#pragma unroll
-                        for (int part = 0; part < HD / 32; ++part) {
-                            tmem_ld32(o_at + 32 * part, s);
-#pragma unroll
-                            for (int k = 0; k < 32; ++k) {
-                                s[k] *= down;
+                        for (int k = 0; k < 16; ++k) {
+                            if (!WHOLE) {
+                                x[k] = 16 * part + k <= hi && 16 * part + k >= lo ? x[k] : -INFINITY;
                             }
-                            tmem_st32(o_at + 32 * part, s);
+                            top4[k & 3] = fmaxf(top4[k & 3], x[k]);
                         }
-                        tmem_wait_st();
+                        tmem_wait_ld(s[(part + 1) & 1]);
                     }
-                }
-                const float ref = m == -INFINITY ? 0.0f : m;
+                    float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
+                    top = top == -INFINITY ? top : top * qs;
+                    const bool higher = top > m + SLACK || (m == -INFINITY && top > m);
+                    if (__any_sync(0xFFFFFFFFu, higher)) {
+                        const float down = higher ? exp2_fast(m - top) : 1.0f;
+                        m = higher ? top : m;
+                        l *= down;
+                        if (kb > 0) {
+                            float (&x)[16] = s[1];
+#pragma unroll 1
+                            for (int part = 0; part < HD / 16; ++part) {
+                                tmem_ld16(o_at + 16 * part, x);
+                                tmem_wait_ld(x);
 #pragma unroll
-                for (int part = 0; part < BLOCK / 32; ++part) {
-                    uint32_t p[16];
-                    tmem_ld32(s_at + 32 * part, s);
-#pragma unroll
-                    for (int k = 0; k < 32; ++k) {
-                        s[k] = exp2_fast(fmaf(s[k], qs, -ref));
-                        if (!whole) {
-                            s[k] = 32 * part + k <= hi && 32 * part + k >= lo ? s[k] : 0.0f;
+                                for (int k = 0; k < 16; ++k) {
+                                    x[k] *= down;
+                                }
+                                tmem_st16(o_at + 16 * part, x);
+                            }
+                            tmem_wait_st();
                         }
                     }
-                    float sum0 = 0.0f, sum1 = 0.0f;
+                    const float ref = m == -INFINITY ? 0.0f : m;
+                    static_assert(PARTS % 2 == 0, "the first part is in s[0] again");
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        sum0 += s[2 * k];
-                        sum1 += s[2 * k + 1];
-                        p[k] = h2_bits(__floats2half2_rn(s[2 * k], s[2 * k + 1]));
+                    for (int part = 0; part < PARTS; ++part) {
+                        float (&x)[16] = s[part & 1];
+                        uint32_t p[8];
+                        if (part + 1 < PARTS) {
+                            tmem_ld16(s_at + 16 * (part + 1), s[(part + 1) & 1]);
+                        }
+                        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) {
+                            x[k] = exp2_fast(fmaf(x[k], qs, -ref));
+                            if (!WHOLE) {
+                                x[k] = 16 * part + k <= hi && 16 * part + k >= lo ? x[k] : 0.0f;
+                            }
+                            sum[k & 3] += x[k];
+                        }
+                        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            p[k] = h2_bits(__floats2half2_rn(x[2 * k], x[2 * k + 1]));
+                        }
+                        if (part + 1 < PARTS) {
+                            tmem_wait_ld(s[(part + 1) & 1]);
+                        }
+                        tmem_st8(s_at + 8 * part, p);  // over columns that have been read
                     }
-                    l += sum0 + sum1;
-                    tmem_st16(s_at + 16 * part, p);  // over columns that have been read
+                    tmem_wait_st();
+                };
+                if (__all_sync(0xFFFFFFFFu, hi >= BLOCK - 1 && lo <= 0)) {
+                    probabilities(std::true_type{});
+                } else {
+                    probabilities(std::false_type{});
                 }
-                tmem_wait_st();
                 // a value that is not finite: its stage is filled before the product that this column's arrival allows
                 const uint32_t b = blocks_before + kb;
                 ok = g_mbar_wait_warp(&ctl.v_full[b & 1], b >> 1 & 1);
-                for (int w = 0; w < KV_WARPS; ++w) {
-                    const uint32_t bits = *reinterpret_cast<volatile uint32_t*>(&ctl.poison[b & 1][w]);
-                    for (int k = 0; bits != 0 && k < KV_TILE; ++k) {
-                        const int key = w * KV_TILE + k;
-                        poisoned |= (bits >> k & 1u) && key <= hi && key >= lo;
+                const uint32_t mine = lane < KV_TILES ? *reinterpret_cast<volatile uint32_t*>(&ctl.poison[b & 1][lane]) : 0u;
+                if (__any_sync(0xFFFFFFFFu, mine != 0)) {
+                    for (int w = 0; w < KV_TILES; ++w) {
+                        const uint32_t bits = __shfl_sync(0xFFFFFFFFu, mine, w);
+                        for (int k = 0; bits != 0 && k < KV_TILE; ++k) {
+                            const int key = w * KV_TILE + k;
+                            poisoned |= (bits >> k & 1u) && key <= hi && key >= lo;
+                        }
                     }
                 }
                 fence_before();
@@ -668,13 +748,16 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
             const int64_t row = it.q.row0 + (it.col0 + c) / a.group;
             const int qh = it.head * a.group + (it.col0 + c) % a.group;
             __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + row * a.out_stride + (int64_t)qh * HD;
-            const bool none = it.blocks[i] == 0 || (m == -INFINITY && l == 0.0f);
+            const bool none = my_blocks == 0 || (m == -INFINITY && l == 0.0f);
             const float inv = none ? 0.0f : poisoned ? __uint_as_float(0x7FC00000u) : 1.0f / l;
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
-                float o[32];
-                if (it.blocks[i] > 0) {
-                    tmem_ld32(o_at + 32 * n, o);
+                float o[2][16];
+                if (my_blocks > 0) {
+                    tmem_ld16(o_at + 32 * n, o[0]);
+                    tmem_ld16(o_at + 32 * n + 16, o[1]);
+                    tmem_wait_ld(o[0]);
+                    tmem_wait_ld(o[1]);
                 }
                 if (c < it.cols && ok) {
 #pragma unroll
@@ -683,7 +766,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
 #pragma unroll
                         for (int h = 0; h < 4; ++h) {
                             const int d = 8 * k + 2 * h, from = 8 * (d & 3) + (d >> 2);
-                            const float x0 = none ? 0.0f : o[from] * inv, x1 = none ? 0.0f : o[from + 8] * inv;
+                            const float x0 = none ? 0.0f : o[from >> 4][from & 15] * inv, x1 = none ? 0.0f : o[(from + 8) >> 4][(from + 8) & 15] * inv;
                             const __nv_bfloat162 pair = __floats2bfloat162_rn(x0, x1);
                             x[h] = *reinterpret_cast<const uint32_t*>(&pair);
                         }
@@ -694,8 +777,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
             fence_before();
         }
         blocks_before += it.most;
-        tile_before[0] += it.blocks[0];
-        tile_before[1] += it.blocks[1];
+        before0 += it.blocks[0];
+        before1 += it.blocks[1];
         ++items_before;
         __syncthreads();
         fence_after();
