@@ -58,12 +58,11 @@ struct Item {
 };
 
 struct Control {
-    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full;
+    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2][2], o_full;  // probabilities: of either half of the keys
     uint32_t tmem;
-    Item item;
-    int item_seq, item_local;
+    Item item[2];                  // the one that is worked on and the next; seq < 0: there is none
     int late;
-    uint32_t poison[2][KV_TILES];  // per stage and tile: tokens whose value is not finite
+    uint32_t poison[8][KV_TILES];  // of the last blocks, per tile: tokens whose value is not finite
     float q_scale[COLS];
 };
 
@@ -141,6 +140,30 @@ __device__ __forceinline__ float exp2_fast(float x)
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Packed pairs of fp32, and the largest of three.
+__device__ __forceinline__ float2 add2(float2 x, float2 y)
+{
+    float2 z;
+    asm("{\n.reg .b64 a, b, c;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nadd.rn.f32x2 c, a, b;\nmov.b64 {%0, %1}, c;\n}"
+        : "=f"(z.x), "=f"(z.y)
+        : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
+    return z;
+}
+__device__ __forceinline__ float2 fma2(float2 x, float2 y, float2 w)
+{
+    float2 z;
+    asm("{\n.reg .b64 a, b, c, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmov.b64 c, {%6, %7};\n"
+        "fma.rn.f32x2 d, a, b, c;\nmov.b64 {%0, %1}, d;\n}"
+        : "=f"(z.x), "=f"(z.y)
+        : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y), "f"(w.x), "f"(w.y));
+    return z;
+}
+__device__ __forceinline__ float max3(float x, float y, float z)
+{
+    float m;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(x), "f"(y), "f"(z));
+    return m;
+}
 // Four 8 x 8 matrices of fp16, rows of 16 bytes: lane 4g + t holds row g, columns 2t and 2t + 1 of each, lane 8m + r names the
 // place of row r of matrix m.
 __device__ __forceinline__ void store_matrices(void* row, const uint32_t (&x)[4])
@@ -176,15 +199,14 @@ __device__ __forceinline__ void quants(const uint32_t* w, uint32_t (&v)[4])
         }
     }
 }
+// Volatile: the loads are issued where they stand (as plain ones they were moved down to their uses, a block later).
 template <int BYTES>
 __device__ __forceinline__ void load_words(uint32_t* w, const uint8_t* p)
 {
     if (BYTES == 16) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
-        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+        asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p));
     } else {
-        const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-        w[0] = v.x, w[1] = v.y;
+        asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
     }
 }
 
@@ -212,7 +234,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
             g_mbar_init(&ctl.k_empty[i], 1);
             g_mbar_init(&ctl.v_empty[i], 1);
             g_mbar_init(&ctl.s_full[i], 1);
-            g_mbar_init(&ctl.p_full[i], 4);
+            g_mbar_init(&ctl.p_full[i][0], 4);
+            g_mbar_init(&ctl.p_full[i][1], 4);
         }
         g_mbar_init(&ctl.o_full, 1);
         ctl.late = 0;
@@ -238,88 +261,94 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
         *reinterpret_cast<volatile int*>(&ctl.late) = 1;
     };
 
-    for (bool first = true;; first = false) {
-        // ---- the next item: heavy ones (late columns) of a sequence first, its kv heads side by side ----
-        if (mma_warp) {
-            unsigned int want = blockIdx.x;
-            if (!first) {
-                if (lane == 0) {
-                    want = gridDim.x + atomicAdd(next_item, 1u);
-                }
-                want = __shfl_sync(0xFFFFFFFFu, want, 0);
-            }
-            long long before = 0;
-            int seq = -1, local = 0;
-            for (int base = 0; base < a.seqs.batch && seq < 0; base += 32) {
-                const int s = base + lane;
-                bool bad = false;
-                long long n = 0;
-                if (s < a.seqs.batch) {
-                    const KvSeq q = kv_seq(a.pool, a.seqs, s, bad);
-                    n = ((long long)q.n * a.group + COLS - 1) / COLS * a.pool.kv_heads;
-                }
-                if (bad && blockIdx.x == 0 && first) {
-                    atomicExch(a.seqs.status, KV_BAD_ROWS);
-                }
-                long long upto = n;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const long long u = __shfl_up_sync(0xFFFFFFFFu, upto, o);
-                    upto += lane >= o ? u : 0;
-                }
-                const bool mine = n > 0 && before + upto - n <= want && want < before + upto;
-                const unsigned int who = __ballot_sync(0xFFFFFFFFu, mine);
-                if (who != 0) {
-                    const int from = __ffs(who) - 1;
-                    seq = base + from;
-                    local = (int)(want - (before + __shfl_sync(0xFFFFFFFFu, upto - n, from)));
-                }
-                before += __shfl_sync(0xFFFFFFFFu, upto, 31);
-            }
+    // The next item, for the warp that issues MMAs: heavy ones (late columns) of a sequence first, its kv heads side by side.
+    auto fetch = [&](Item& to, bool first) {
+        unsigned int want = blockIdx.x;
+        if (!first) {
             if (lane == 0) {
-                ctl.item_seq = seq;
-                ctl.item_local = local;
+                want = gridDim.x + atomicAdd(next_item, 1u);
             }
+            want = __shfl_sync(0xFFFFFFFFu, want, 0);
         }
-        __syncthreads();
-        if (ctl.item_seq < 0 || ctl.late) {
+        long long before = 0;
+        int seq = -1, local = 0;
+        for (int base = 0; base < a.seqs.batch && seq < 0; base += 32) {
+            const int s = base + lane;
+            bool bad = false;
+            long long n = 0;
+            if (s < a.seqs.batch) {
+                const KvSeq q = kv_seq(a.pool, a.seqs, s, bad);
+                n = ((long long)q.n * a.group + COLS - 1) / COLS * a.pool.kv_heads;
+            }
+            if (bad && blockIdx.x == 0 && first) {
+                atomicExch(a.seqs.status, KV_BAD_ROWS);
+            }
+            long long upto = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long u = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+                upto += lane >= o ? u : 0;
+            }
+            const bool mine = n > 0 && before + upto - n <= want && want < before + upto;
+            const unsigned int who = __ballot_sync(0xFFFFFFFFu, mine);
+            if (who != 0) {
+                const int from = __ffs(who) - 1;
+                seq = base + from;
+                local = (int)(want - (before + __shfl_sync(0xFFFFFFFFu, upto - n, from)));
+            }
+            before += __shfl_sync(0xFFFFFFFFu, upto, 31);
+        }
+        if (lane == 0) {
+            Item n = {};
+            n.seq = seq;
+            if (seq >= 0) {
+                bool bad;
+                n.q = kv_seq(a.pool, a.seqs, n.seq, bad);
+                const long long columns = (long long)n.q.n * a.group;
+                const int tiles = (int)((columns + COLS - 1) / COLS);
+                const int tile = tiles - 1 - local / a.pool.kv_heads;
+                n.head = local % a.pool.kv_heads;
+                n.col0 = tile * COLS;
+                n.cols = (int)min((long long)COLS, columns - n.col0);
+                n.first_pos = n.q.len - n.q.n;
+                const int pos_lo = n.first_pos + n.col0 / a.group;
+                n.pos_hi = n.first_pos + (n.col0 + n.cols - 1) / a.group;
+                n.seen_lo = a.window > 0 ? max(0, pos_lo - a.window + 1) : 0;
+                n.k0 = n.seen_lo / KV_TILE * KV_TILE;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int last = min(n.cols, (i + 1) * M_TILE) - 1;  // the M tile's last column
+                    const int pos = n.first_pos + (n.col0 + last) / a.group;
+                    n.blocks[i] = last < i * M_TILE || pos < n.k0 ? 0 : (pos - n.k0) / BLOCK + 1;
+                }
+                n.most = max(n.blocks[0], n.blocks[1]);
+            }
+            to = n;
+        }
+        __syncwarp();
+    };
+    if (mma_warp) {
+        fetch(ctl.item[0], true);
+    }
+    __syncthreads();
+
+    for (;;) {
+        const Item& it = ctl.item[items_before & 1];
+        if (it.seq < 0 || ctl.late) {
             break;
         }
-        const Item& it = ctl.item;
-        if (threadIdx.x == 0) {
-            Item n;
-            bool bad;
-            n.seq = ctl.item_seq;
-            n.q = kv_seq(a.pool, a.seqs, n.seq, bad);
-            const long long columns = (long long)n.q.n * a.group;
-            const int tiles = (int)((columns + COLS - 1) / COLS);
-            const int tile = tiles - 1 - ctl.item_local / a.pool.kv_heads;
-            n.head = ctl.item_local % a.pool.kv_heads;
-            n.col0 = tile * COLS;
-            n.cols = (int)min((long long)COLS, columns - n.col0);
-            n.first_pos = n.q.len - n.q.n;
-            const int pos_lo = n.first_pos + n.col0 / a.group;
-            n.pos_hi = n.first_pos + (n.col0 + n.cols - 1) / a.group;
-            n.seen_lo = a.window > 0 ? max(0, pos_lo - a.window + 1) : 0;
-            n.k0 = n.seen_lo / KV_TILE * KV_TILE;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int last = min(n.cols, (i + 1) * M_TILE) - 1;  // the M tile's last column
-                const int pos = n.first_pos + (n.col0 + last) / a.group;
-                n.blocks[i] = last < i * M_TILE || pos < n.k0 ? 0 : (pos - n.k0) / BLOCK + 1;
-            }
-            n.most = max(n.blocks[0], n.blocks[1]);
-            ctl.item = n;
+        if (mma_warp) {  // while the others load queries
+            fetch(ctl.item[(items_before & 1) ^ 1], false);
         }
-        __syncthreads();
         // ---- queries ----
-        if (warp < SOFT_WARPS) {
-            constexpr int EACH = HD / 32;  // consecutive dimensions of a lane
-            for (int c4 = 0; c4 < 32; c4 += 4) {
-                float v[4][EACH];
+        else {
+            constexpr int EACH = HD / 32, AT_ONCE = 8;  // consecutive dimensions of a lane, columns in flight
+            constexpr int MINE = COLS / (SOFT_WARPS + KV_WARPS);
+            for (int c8 = 0; c8 < MINE; c8 += AT_ONCE) {
+                float v[AT_ONCE][EACH];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int c = warp * 32 + c4 + k;
+                for (int k = 0; k < AT_ONCE; ++k) {
+                    const int c = warp * MINE + c8 + k;
                     const bool on = c < it.cols;
                     const int64_t row = it.q.row0 + (on ? (it.col0 + c) / a.group : 0);
                     const int qh = it.head * a.group + (on ? (it.col0 + c) % a.group : 0);
@@ -339,8 +368,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
                     }
                 }
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int c = warp * 32 + c4 + k;
+                for (int k = 0; k < AT_ONCE; ++k) {
+                    const int c = warp * MINE + c8 + k;
                     uint32_t bits = 0;
 #pragma unroll
                     for (int i = 0; i < EACH; ++i) {
@@ -353,8 +382,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
                     uint8_t* row = q_smem + (c / M_TILE) * Shape::Q_BYTES + (c % M_TILE) * 128;
 #pragma unroll
                     for (int i = 0; i < EACH; i += 2) {
-                        const int dim = lane * EACH + i, chunk = (dim % 64) / 8;
-                        *reinterpret_cast<__half2*>(row + dim / 64 * (M_TILE * 128) + ((chunk ^ (c & 7)) << 4) + dim % 8 * 2) =
+                        // dimension 32 n + 8 t + 2 r + e lies at 32 n + 8 r + 2 t + e, as in the keys
+                        const int dim = lane * EACH + i, chunk = (dim % 64) / 32 * 4 + dim / 2 % 4;
+                        *reinterpret_cast<__half2*>(row + dim / 64 * (M_TILE * 128) + ((chunk ^ (c & 7)) << 4) + dim / 8 % 4 * 4) =
                             __floats2half2_rn(v[k][i] * up, v[k][i + 1] * up);
                     }
                     if (lane == 0) {
@@ -389,12 +419,12 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
                 }
                 __syncwarp();
             };
-            auto values = [&](int i, int kb) {
+            auto values = [&](int i, int kb, int half) {
                 const uint32_t stage = (blocks_before + kb) & 1;
                 fence_after();
                 if (elect_one()) {
 #pragma unroll
-                    for (int kk = 0; kk < BLOCK / 16; ++kk) {
+                    for (int kk = half * BLOCK / 32; kk < (half + 1) * BLOCK / 32; ++kk) {
                         umma_ts(tmem + 2 * BLOCK + i * M_TILE, tmem + i * BLOCK + 8 * kk,
                                 v_desc + (uint64_t)((stage * Shape::V_BYTES + (kk >> 2) * HD * 128) >> 4) + 2 * (kk & 3), id_o,
                                 kb > 0 || kk > 0);
@@ -429,9 +459,12 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
                 for (int i = 0; i < 2; ++i) {
                     const int mine = i ? blocks1 : blocks0;
                     if (kb < mine && ok) {
-                        wait(&ctl.p_full[i], ((i ? before1 : before0) + kb) & 1);
-                        if (ok) {
-                            values(i, kb);
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            wait(&ctl.p_full[i][half], ((i ? before1 : before0) + kb) & 1);
+                            if (ok) {
+                                values(i, kb, half);
+                            }
                         }
                     }
                     if (kb + 1 < mine && ok) {
@@ -513,7 +546,6 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
                 if (ok) {
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        const int key = w * KV_TILE + 8 * j + g;
 #pragma unroll
                         for (int n = 0; n < NB; ++n) {
                             uint32_t x[4];
@@ -526,9 +558,12 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
                                     x[i] = h2_bits(__hmul2(as_h2(x[i]), d));
                                 }
                             }
-                            const int chunk = 4 * (n & 1) + t;  // dimensions 32 n + 8 t .. of the key's row
-                            *reinterpret_cast<uint4*>(k_smem + stage * Shape::K_BYTES + (n >> 1) * BLOCK * 128 + key * 128 +
-                                                      ((chunk ^ g) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
+                            // matrix r: keys g, dimensions 32 n + 8 t + 2 r + {0, 1}.  This lane's row for the store is key
+                            // lane & 7, its 16 bytes are matrix lane >> 3
+                            const int row = w * KV_TILE + 8 * j + (lane & 7), chunk = 4 * (n & 1) + (lane >> 3);
+                            store_matrices(k_smem + stage * Shape::K_BYTES + (n >> 1) * BLOCK * 128 + row * 128 +
+                                               ((chunk ^ (lane & 7)) << 4),
+                                           x);
                         }
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -609,7 +644,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
                         put(std::false_type{}, all);
                     }
                     if (lane == 0) {
-                        ctl.poison[stage][w] = poison;
+                        ctl.poison[b & 7][w] = poison;
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
@@ -633,6 +668,21 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
             float m = -INFINITY, l = 0.0f;
             bool ok = true, poisoned = false;
             const int my_blocks = it.blocks[i];
+            // whether this column sees a value of block kb that is not finite.  The block's words stay for eight blocks, and
+            // the warps that write them are at most two ahead of the values that are multiplied
+            auto look_for_poison = [&](int kb) {
+                const uint32_t mine =
+                    lane < KV_TILES ? *reinterpret_cast<volatile uint32_t*>(&ctl.poison[(blocks_before + kb) & 7][lane]) : 0u;
+                if (__any_sync(0xFFFFFFFFu, mine != 0)) {
+                    for (int w = 0; w < KV_TILES; ++w) {
+                        const uint32_t bits = __shfl_sync(0xFFFFFFFFu, mine, w);
+                        for (int k = 0; bits != 0 && k < KV_TILE; ++k) {
+                            const int key = it.k0 + kb * BLOCK + w * KV_TILE + k;
+                            poisoned |= (bits >> k & 1u) && key <= pos && key >= low;
+                        }
+                    }
+                }
+            };
             const uint32_t my_before = i ? before1 : before0;
             for (int kb = 0; kb < my_blocks && ok; ++kb) {
                 const int key0 = it.k0 + kb * BLOCK;
@@ -654,16 +704,19 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
                     for (int part = 0; part < PARTS; ++part) {
                         float (&x)[16] = s[part & 1];
                         tmem_ld16(s_at + 16 * ((part + 1) % PARTS), s[(part + 1) & 1]);
+                        if (!WHOLE) {
 #pragma unroll
-                        for (int k = 0; k < 16; ++k) {
-                            if (!WHOLE) {
+                            for (int k = 0; k < 16; ++k) {
                                 x[k] = 16 * part + k <= hi && 16 * part + k >= lo ? x[k] : -INFINITY;
                             }
-                            top4[k & 3] = fmaxf(top4[k & 3], x[k]);
+                        }
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            top4[k & 3] = max3(top4[k & 3], x[2 * k], x[2 * k + 1]);
                         }
                         tmem_wait_ld(s[(part + 1) & 1]);
                     }
-                    float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
+                    float top = fmaxf(top4[0], max3(top4[1], top4[2], top4[3]));
                     top = top == -INFINITY ? top : top * qs;
                     const bool higher = top > m + SLACK || (m == -INFINITY && top > m);
                     if (__any_sync(0xFFFFFFFFu, higher)) {
@@ -687,6 +740,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
                     }
                     const float ref = m == -INFINITY ? 0.0f : m;
                     static_assert(PARTS % 2 == 0, "the first part is in s[0] again");
+                    float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
                     for (int part = 0; part < PARTS; ++part) {
                         float (&x)[16] = s[part & 1];
@@ -694,25 +748,32 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
                         if (part + 1 < PARTS) {
                             tmem_ld16(s_at + 16 * (part + 1), s[(part + 1) & 1]);
                         }
-                        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) {
-                            x[k] = exp2_fast(fmaf(x[k], qs, -ref));
-                            if (!WHOLE) {
-                                x[k] = 16 * part + k <= hi && 16 * part + k >= lo ? x[k] : 0.0f;
-                            }
-                            sum[k & 3] += x[k];
-                        }
-                        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 #pragma unroll
                         for (int k = 0; k < 8; ++k) {
-                            p[k] = h2_bits(__floats2half2_rn(x[2 * k], x[2 * k + 1]));
+                            const float2 y = fma2(make_float2(x[2 * k], x[2 * k + 1]), make_float2(qs, qs), make_float2(-ref, -ref));
+                            float2 e = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+                            if (!WHOLE) {
+                                e.x = 16 * part + 2 * k <= hi && 16 * part + 2 * k >= lo ? e.x : 0.0f;
+                                e.y = 16 * part + 2 * k + 1 <= hi && 16 * part + 2 * k + 1 >= lo ? e.y : 0.0f;
+                            }
+                            sum[k & 1] = add2(sum[k & 1], e);
+                            p[k] = h2_bits(__floats2half2_rn(e.x, e.y));
                         }
                         if (part + 1 < PARTS) {
                             tmem_wait_ld(s[(part + 1) & 1]);
                         }
                         tmem_st8(s_at + 8 * part, p);  // over columns that have been read
+                        if (part == PARTS / 2 - 1) {  // the first half of the product can begin
+                            tmem_wait_st();
+                            fence_before();
+                            __syncwarp();
+                            if (lane == 0) {
+                                g_mbar_arrive(&ctl.p_full[i][0]);
+                            }
+                        }
                     }
+                    sum[0] = add2(sum[0], sum[1]);
+                    l += sum[0].x + sum[0].y;
                     tmem_wait_st();
                 };
                 if (__all_sync(0xFFFFFFFFu, hi >= BLOCK - 1 && lo <= 0)) {
@@ -720,23 +781,13 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
                 } else {
                     probabilities(std::false_type{});
                 }
-                // a value that is not finite: its stage is filled before the product that this column's arrival allows
-                const uint32_t b = blocks_before + kb;
-                ok = g_mbar_wait_warp(&ctl.v_full[b & 1], b >> 1 & 1);
-                const uint32_t mine = lane < KV_TILES ? *reinterpret_cast<volatile uint32_t*>(&ctl.poison[b & 1][lane]) : 0u;
-                if (__any_sync(0xFFFFFFFFu, mine != 0)) {
-                    for (int w = 0; w < KV_TILES; ++w) {
-                        const uint32_t bits = __shfl_sync(0xFFFFFFFFu, mine, w);
-                        for (int k = 0; bits != 0 && k < KV_TILE; ++k) {
-                            const int key = w * KV_TILE + k;
-                            poisoned |= (bits >> k & 1u) && key <= hi && key >= lo;
-                        }
-                    }
-                }
                 fence_before();
                 __syncwarp();
                 if (lane == 0) {
-                    g_mbar_arrive(&ctl.p_full[i]);
+                    g_mbar_arrive(&ctl.p_full[i][1]);
+                }
+                if (kb > 0) {  // this block's scores were issued behind the last one's values, which were complete by then
+                    look_for_poison(kb - 1);
                 }
             }
             // ---- results ----
@@ -745,6 +796,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
                 give_up();
             }
             fence_after();
+            if (ok && my_blocks > 0) {
+                look_for_poison(my_blocks - 1);
+            }
             const int64_t row = it.q.row0 + (it.col0 + c) / a.group;
             const int qh = it.head * a.group + (it.col0 + c) % a.group;
             __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + row * a.out_stride + (int64_t)qh * HD;
@@ -779,8 +833,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
         blocks_before += it.most;
         before0 += it.blocks[0];
         before1 += it.blocks[1];
-        ++items_before;
         __syncthreads();
+        ++items_before;
         fence_after();
     }
 
