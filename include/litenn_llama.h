@@ -19,6 +19,7 @@
 #ifndef LITENN_LLAMA_H
 #define LITENN_LLAMA_H
 
+#include "litenn_kv.h"
 #include "litenn_qmm.h"
 
 #ifdef __cplusplus
@@ -77,6 +78,11 @@ int qmm_llama_set_embedding(qmm_llama* m, const void* payload_host, size_t paylo
  * (tools/gguf/LLaMABuilder.cpp:719-733).  Packs this rank's rows of the embedding payload as the
  * output weight; the model owns the packed copy.  Use instead of qmm_llama_set_weight(QMM_LL_HEAD). */
 int qmm_llama_tie_output(qmm_llama* m, const void* embedding_payload_host, size_t payload_bytes, void* stream);
+
+/* Rotary positions of models whose context has been stretched (GGUF: rope.scaling.* and the tensor rope_freqs.weight, whose
+ * rope_dim / 2 values go to freq_factors_host; either may be NULL).  Frequencies as by qmm_rope_frequencies from the
+ * configuration's theta.  Before the first token; every path of the model follows. */
+int qmm_llama_set_rope_scaling(qmm_llama* m, const float* freq_factors_host, const qmm_rope_scaling* scaling);
 
 /* Tensor-parallel set-up.  Rank 0 obtains an id (128 bytes) and hands it to every rank by
  * any host channel; every rank then calls qmm_llama_tp_init with the same id. */
@@ -158,6 +164,14 @@ int qmm_llama_last_logits(qmm_llama* m, float* logits_host, void* stream);
  *   _decode_enqueue / _generated_tokens   the same without / only the copy to the host
  */
 int qmm_llama_batch_create(qmm_llama* m, int batch, int max_steps);
+/*
+ * The same batch over a paged cache (litenn_kv.h): `n_pages` pages of `page_tokens` tokens (a multiple of 16) in every block,
+ * fp16, Q8_0 or Q4_0 (kv_fmt), which the sequences take as they grow, instead of max_seq positions of fp16 each.  Prompts
+ * append and attend in pages as well.  A call that would need more pages than are free is refused (QMM_E_INVALID) before
+ * it does anything; qmm_llama_reset frees all of them.
+ */
+int qmm_llama_batch_create_paged(qmm_llama* m, int batch, int max_steps, int kv_fmt, int page_tokens, int64_t n_pages);
+int qmm_llama_batch_free_pages(const qmm_llama* m, int64_t* free_pages);
 int qmm_llama_batch_prefill(qmm_llama* m, int seq, const int32_t* tokens_host, int n, int32_t* first_token_out,
                             void* stream);
 int qmm_llama_batch_decode(qmm_llama* m, int steps, int32_t* tokens_out_host, void* stream);

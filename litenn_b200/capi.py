@@ -107,6 +107,9 @@ LLAMA_SYMBOLS = {
     "qmm_llama_has_graph": (_i, [_vp]),
     "qmm_llama_generated_tokens": (_i, [_vp, _i, _i, _vp, _vp]),
     "qmm_llama_batch_create": (_i, [_vp, _i, _i]),
+    "qmm_llama_batch_create_paged": (_i, [_vp, _i, _i, _i, _i, _i64]),
+    "qmm_llama_batch_free_pages": (_i, [_vp, ctypes.POINTER(_i64)]),
+    "qmm_llama_set_rope_scaling": (_i, [_vp, _vp, _vp]),
     "qmm_llama_batch_prefill": (_i, [_vp, _i, _vp, _i, _vp, _vp]),
     "qmm_llama_batch_decode": (_i, [_vp, _i, _vp, _vp]),
     "qmm_llama_batch_decode_enqueue": (_i, [_vp, _i, _vp]),

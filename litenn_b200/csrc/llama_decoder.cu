@@ -18,13 +18,15 @@
 // 1/rms commutes with the matvec.)  With tensor parallelism the two K-split matvecs also exchange their
 // partial sums with the peers inside that epilogue (PeerScatter, qmm_common.cuh); with NCCL sums instead,
 // a stand-alone kernel does the residual add and the packing after the all-reduce.
-// Batched decode (enqueue_batch_step) is the row form of the same chain.
+// Batched decode (enqueue_batch_step) is the row form of the same chain; with a paged cache (litenn_kv.h) its attention is an append, an
+// attention and a packing kernel instead of the fused one, and its pages are handed out here.
 #include "../../include/litenn_llama.h"
 
 #include <dlfcn.h>
 
 #include <algorithm>
 #include <chrono>
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <string>
@@ -141,6 +143,17 @@ struct qmm_llama {
     std::vector<int> bpos_host, btok_host;
     int bsteps_host = 0;
     cudaGraphExec_t bgraph = nullptr;
+    // paged batch (qmm_llama_batch_create_paged): a pool per block, page numbers shared by all blocks
+    bool paged = false;
+    qmm_kv_cache bkv = {};                 // pool_dev is filled in per block
+    std::vector<uint8_t*> bpool;
+    int bwidth = 0;                        // page numbers per sequence
+    int *btable = nullptr, *blen = nullptr, *prompt_rows = nullptr;  // [batch][bwidth], [batch], {0, rows, length}
+    std::vector<int> btable_host, bheld, bfree;
+    float* bctx = nullptr;
+    uint8_t* bwork = nullptr;
+    double* rope_freq = nullptr;           // [rope_dim / 2], what the tables hold the angles of
+    double rope_gain = 1.0;
     // The peer exchange numbers its arg-max packets by position, which repeats when the sequences of a batch
     // are prefilled one after another: those prefills gather their candidates with NCCL instead.
     bool pick_with_nccl = false;
@@ -472,6 +485,51 @@ void drop_graph(qmm_llama* m)
     }
 }
 
+qmm_rope rope_of(const qmm_llama* m)
+{
+    return {m->cfg.rope_dim, QMM_ROPE_PAIRS, m->rope_freq, m->rope_gain};
+}
+
+// Rotates, appends and attends rows [q | k | v] of a paged batch's sequences in block l; the context goes to `out`.
+int paged_attention(qmm_llama* m, int l, const qmm_kv_batch& rows, float* qkv, void* out, int out_type, cudaStream_t st)
+{
+    const int hd = m->cfg.head_dim;
+    const int64_t stride = (int64_t)(m->hl + 2 * m->kvl) * hd, ctx_w = (int64_t)m->hl * hd;
+    const qmm_rope rope = rope_of(m);
+    qmm_kv_cache cache = m->bkv;
+    cache.pool_dev = m->bpool[l];
+    float *k = qkv + ctx_w, *v = k + (int64_t)m->kvl * hd;
+    LL_QMM(qmm_kv_append(m->device, &cache, &rows, &rope, m->hl, QMM_OUT_F32, qkv, stride, k, stride, v, stride, qkv, QMM_OUT_F32,
+                         stride, st));
+    return qmm_kv_attention(m->device, &cache, &rows, m->hl, qkv, QMM_OUT_F32, stride, out, out_type, ctx_w,
+                            1.0f / sqrtf((float)hd), 0, m->bwork, st);
+}
+
+// Pages for `tokens[s]` tokens of every sequence, or none at all.
+int reserve_pages(qmm_llama* m, const std::vector<int>& tokens, cudaStream_t st)
+{
+    size_t want = 0;
+    for (int s = 0; s < m->batch; ++s) {
+        want += (size_t)std::max(0, (tokens[s] + m->bkv.page_tokens - 1) / m->bkv.page_tokens - m->bheld[s]);
+    }
+    if (want > m->bfree.size()) {
+        char buf[120];
+        snprintf(buf, sizeof buf, "the cache has %zu free pages and the call needs %zu", m->bfree.size(), want);
+        return qmm_internal_fail(QMM_E_INVALID, buf);
+    }
+    if (want == 0) {
+        return QMM_OK;
+    }
+    for (int s = 0; s < m->batch; ++s) {
+        while (m->bheld[s] * m->bkv.page_tokens < tokens[s]) {
+            m->btable_host[(size_t)s * m->bwidth + m->bheld[s]++] = m->bfree.back();
+            m->bfree.pop_back();
+        }
+    }
+    LL_CUDA(cudaMemcpyAsync(m->btable, m->btable_host.data(), m->btable_host.size() * sizeof(int), cudaMemcpyHostToDevice, st));
+    return QMM_OK;
+}
+
 // One step of `batch` sequences: every sequence's current token -> its next token.  The linears see the
 // batch as the rows of one skinny product (packed matvec at batch 2..16); attention, position and cache
 // are per sequence.  Whatever feeds a linear packs its own result, so a block is eight launches (twelve with
@@ -481,17 +539,26 @@ int enqueue_batch_step(qmm_llama* m, cudaStream_t st)
     const qmm_llama_config& c = m->cfg;
     const int B = m->batch, d = c.d_model, hd = c.head_dim;
     LL_CUDA(ll_embed_rows(c.embd_fmt, m->embd, m->btok, B, d, m->bh, st));
+    if (m->paged) {
+        LL_CUDA(ll_next_lengths(m->bpos, B, m->blen, st));
+    }
     for (int l = 0; l < c.n_layers; ++l) {
         Layer& L = m->layers[l];
         LL_CUDA(ll_resid_rmsnorm_rows_packed(m->bh, l == 0 ? nullptr : m->by, L.attn_norm, c.rms_eps, d, B, m->bpk_d, st));
         LL_QMM(qmm_gemv_packed(L.w[QMM_LL_QKV], m->bpk_d, m->bqkv, B, st));
-        AttnBatch ab = {};
-        ab.qkv_stride = (m->hl + 2 * m->kvl) * hd;
-        ab.cache_stride = (int64_t)m->kvl * c.max_seq * hd;
-        ab.packed = m->bpk_ctx;
-        ab.ncp = B == 1 ? 0 : xpack_ncp(B);
-        LL_CUDA(ll_attn_fused(m->bqkv, m->bpos, m->hl, m->kvl, hd, c.rope_dim, m->rope_cos, m->rope_sin, c.max_seq,
-                              m->bcache_k[l], m->bcache_v[l], nullptr, B, ab, st));
+        if (m->paged) {
+            const qmm_kv_batch rows = {B, m->bwidth, m->btable, m->blen, nullptr, B};
+            LL_QMM(paged_attention(m, l, rows, m->bqkv, m->bctx, QMM_OUT_F32, st));
+            LL_QMM(qmm_pack_activations(m->device, m->bctx, B, (int64_t)m->hl * hd, m->bpk_ctx, st));
+        } else {
+            AttnBatch ab = {};
+            ab.qkv_stride = (m->hl + 2 * m->kvl) * hd;
+            ab.cache_stride = (int64_t)m->kvl * c.max_seq * hd;
+            ab.packed = m->bpk_ctx;
+            ab.ncp = B == 1 ? 0 : xpack_ncp(B);
+            LL_CUDA(ll_attn_fused(m->bqkv, m->bpos, m->hl, m->kvl, hd, c.rope_dim, m->rope_cos, m->rope_sin, c.max_seq,
+                                  m->bcache_k[l], m->bcache_v[l], nullptr, B, ab, st));
+        }
         LL_QMM(qmm_gemv_packed(L.w[QMM_LL_O], m->bpk_ctx, m->by, B, st));
         LL_QMM(all_reduce(m, m->by, (size_t)B * d, st));
         LL_CUDA(ll_resid_rmsnorm_rows_packed(m->bh, m->by, L.ffn_norm, c.rms_eps, d, B, m->bpk_d, st));
@@ -608,6 +675,14 @@ int qmm_llama_create(int device, const qmm_llama_config* cfg, qmm_llama** out)
     LL_TRY(dev_alloc(m, &m->pk_act, xpack1_bytes((m->ffl + 255) / 256)));  // zeroed: blocks past ffl stay zero
     LL_TRY(dev_alloc(m, &m->rope_cos, (size_t)c.max_seq * (c.rope_dim / 2)));
     LL_TRY(dev_alloc(m, &m->rope_sin, (size_t)c.max_seq * (c.rope_dim / 2)));
+    LL_TRY(dev_alloc(m, &m->rope_freq, (size_t)c.rope_dim / 2));
+    {
+        std::vector<double> freq((size_t)c.rope_dim / 2);
+        LL_TRY(qmm_rope_frequencies(c.rope_dim, (double)c.rope_theta, nullptr, nullptr, freq.data(), &m->rope_gain));
+        if (rc == QMM_OK && cudaMemcpy(m->rope_freq, freq.data(), freq.size() * sizeof(double), cudaMemcpyHostToDevice) != cudaSuccess) {
+            rc = qmm_internal_fail(QMM_E_CUDA, "copying the rotary frequencies failed");
+        }
+    }
     LL_TRY(dev_alloc(m, &m->pos, 1));
     LL_TRY(dev_alloc(m, &m->token, 1));
     LL_TRY(dev_alloc(m, &m->out_tokens, (size_t)c.max_seq + 8));
@@ -738,6 +813,32 @@ int qmm_llama_set_norm(qmm_llama* m, int layer, int which, const float* weights_
     }
     LL_GUARD(m);
     LL_CUDA(cudaMemcpy(dst, weights_host, (size_t)m->cfg.d_model * sizeof(float), cudaMemcpyHostToDevice));
+    return QMM_OK;
+}
+
+int qmm_llama_set_rope_scaling(qmm_llama* m, const float* freq_factors_host, const qmm_rope_scaling* scaling)
+{
+    if (!m) {
+        return qmm_internal_fail(QMM_E_INVALID, "model handle is null");
+    }
+    bool used = m->host_pos != 0 || m->bsteps_host != 0;
+    for (int p : m->bpos_host) {
+        used = used || p != 0;
+    }
+    if (used) {
+        return qmm_internal_fail(QMM_E_INVALID, "qmm_llama_set_rope_scaling: the cache already holds tokens (qmm_llama_reset first)");
+    }
+    const qmm_llama_config& c = m->cfg;
+    std::vector<double> freq((size_t)c.rope_dim / 2);
+    double gain = 1.0;
+    LL_QMM(qmm_rope_frequencies(c.rope_dim, (double)c.rope_theta, freq_factors_host, scaling, freq.data(), &gain));
+    LL_GUARD(m);
+    LL_CUDA(cudaDeviceSynchronize());
+    LL_CUDA(cudaMemcpy(m->rope_freq, freq.data(), freq.size() * sizeof(double), cudaMemcpyHostToDevice));
+    LL_CUDA(ll_rope_tables_from(c.max_seq, c.rope_dim, m->rope_freq, gain, m->rope_cos, m->rope_sin, nullptr));
+    LL_CUDA(cudaDeviceSynchronize());
+    m->rope_gain = gain;
+    drop_graph(m);  // a paged batch's graph holds the gain
     return QMM_OK;
 }
 
@@ -924,6 +1025,11 @@ int qmm_llama_reset(qmm_llama* m, void* stream)
         LL_CUDA(cudaMemsetAsync(m->bsteps, 0, sizeof(int), st));
         std::fill(m->bpos_host.begin(), m->bpos_host.end(), 0);
         m->bsteps_host = 0;
+        for (int s = 0; m->paged && s < m->batch; ++s) {
+            for (; m->bheld[s] > 0; --m->bheld[s]) {
+                m->bfree.push_back(m->btable_host[(size_t)s * m->bwidth + m->bheld[s] - 1]);
+            }
+        }
     }
     LL_QMM(rearm_exchange(m, st));
     LL_QMM(sync_with_collectives(m, st));
@@ -932,7 +1038,8 @@ int qmm_llama_reset(qmm_llama* m, void* stream)
     return QMM_OK;
 }
 
-int qmm_llama_prefill(qmm_llama* m, const int32_t* tokens_host, int n, int32_t* first_token_out, void* stream)
+// `paged_seq`: the sequence of a paged batch whose pages the prompt goes to, -1 for the layers' own caches.
+static int prefill_rows(qmm_llama* m, const int32_t* tokens_host, int n, int32_t* first_token_out, int paged_seq, void* stream)
 {
     LL_QMM(check_ready(m));
     const qmm_llama_config& c = m->cfg;
@@ -952,14 +1059,24 @@ int qmm_llama_prefill(qmm_llama* m, const int32_t* tokens_host, int n, int32_t* 
     const bool keep_order = d <= 2048;
     LL_CUDA(cudaMemcpyAsync(m->tokens_dev, tokens_host, (size_t)n * sizeof(int), cudaMemcpyHostToDevice, st));
     LL_CUDA(ll_embed_rows(c.embd_fmt, m->embd, m->tokens_dev, n, d, m->hr, st));
+    qmm_kv_batch paged_rows = {};
+    if (paged_seq >= 0) {
+        const int rows[3] = {0, n, n};
+        LL_CUDA(cudaMemcpyAsync(m->prompt_rows, rows, sizeof rows, cudaMemcpyHostToDevice, st));
+        paged_rows = {1, m->bwidth, m->btable + (size_t)paged_seq * m->bwidth, m->prompt_rows + 2, m->prompt_rows, n};
+    }
     for (int l = 0; l < c.n_layers; ++l) {
         Layer& L = m->layers[l];
         LL_CUDA(ll_resid_rmsnorm_rows(m->hr, l == 0 ? nullptr : m->y2r, L.attn_norm, c.rms_eps, d, n, m->xn, st));
         LL_QMM(qmm_internal_gemm(L.w[QMM_LL_QKV], m->xn, m->qkvr, n, GEMM_OUT_F32, keep_order, st));
-        LL_CUDA(ll_rope_kv(m->qkvr, m->pos, 0, n, m->hl, m->kvl, hd, c.rope_dim, m->rope_cos, m->rope_sin, c.max_seq,
-                           L.cache_k, L.cache_v, st));
-        LL_CUDA(ll_attn_prefill(m->qkvr, n, pos0, m->hl, m->kvl, hd, c.max_seq, L.cache_k, L.cache_v, m->ctx,
-                                keep_order ? 256 : 32, st));
+        if (paged_seq >= 0) {
+            LL_QMM(paged_attention(m, l, paged_rows, m->qkvr, m->ctx, QMM_OUT_BF16, st));
+        } else {
+            LL_CUDA(ll_rope_kv(m->qkvr, m->pos, 0, n, m->hl, m->kvl, hd, c.rope_dim, m->rope_cos, m->rope_sin, c.max_seq,
+                               L.cache_k, L.cache_v, st));
+            LL_CUDA(ll_attn_prefill(m->qkvr, n, pos0, m->hl, m->kvl, hd, c.max_seq, L.cache_k, L.cache_v, m->ctx,
+                                    keep_order ? 256 : 32, st));
+        }
         LL_QMM(qmm_internal_gemm(L.w[QMM_LL_O], m->ctx, m->yr, n, GEMM_OUT_F32, keep_order, st));
         LL_QMM(all_reduce(m, m->yr, (size_t)n * d, st));
         LL_CUDA(ll_resid_rmsnorm_rows(m->hr, m->yr, L.ffn_norm, c.rms_eps, d, n, m->xn, st));
@@ -983,6 +1100,11 @@ int qmm_llama_prefill(qmm_llama* m, const int32_t* tokens_host, int n, int32_t* 
         *first_token_out = tok;
     }
     return QMM_OK;
+}
+
+int qmm_llama_prefill(qmm_llama* m, const int32_t* tokens_host, int n, int32_t* first_token_out, void* stream)
+{
+    return prefill_rows(m, tokens_host, n, first_token_out, -1, stream);
 }
 
 int qmm_llama_decode_enqueue(qmm_llama* m, int steps, void* stream)
@@ -1079,7 +1201,8 @@ int qmm_llama_has_graph(const qmm_llama* m)
 
 // ---- batched decode ---------------------------------------------------------------------------------
 
-int qmm_llama_batch_create(qmm_llama* m, int batch, int max_steps)
+// page_tokens 0: contiguous fp16 caches.
+static int batch_create(qmm_llama* m, int batch, int max_steps, int kv_fmt, int page_tokens, int64_t n_pages)
 {
     LL_QMM(check_ready(m));
     if (m->batch != 0) {
@@ -1088,8 +1211,14 @@ int qmm_llama_batch_create(qmm_llama* m, int batch, int max_steps)
     if (batch < 1 || batch > QMM_GEMV_MAX_BATCH || max_steps < 1) {
         return qmm_internal_fail(QMM_E_INVALID, "qmm_llama_batch_create: batch outside 1..16 or no steps");
     }
-    LL_GUARD(m);
     const qmm_llama_config& c = m->cfg;
+    const bool paged = page_tokens != 0;
+    size_t pool_bytes = 0;
+    if (paged) {
+        m->bkv = {kv_fmt, m->kvl, c.head_dim, page_tokens, n_pages, nullptr};
+        LL_QMM(qmm_kv_pool_bytes(&m->bkv, &pool_bytes));
+    }
+    LL_GUARD(m);
     const size_t B = (size_t)batch, d = (size_t)c.d_model, hd = (size_t)c.head_dim;
     const size_t qkv_w = (size_t)(m->hl + 2 * m->kvl) * hd, ctx_w = (size_t)m->hl * hd;
     auto alloc_packed = [&](uint8_t** p, size_t width) -> int {
@@ -1111,17 +1240,59 @@ int qmm_llama_batch_create(qmm_llama* m, int batch, int max_steps)
     LL_QMM(dev_alloc(m, &m->bsteps, 1));
     LL_QMM(dev_alloc(m, &m->bpair, B * 2 * ARGMAX_CTAS));
     LL_QMM(dev_alloc(m, &m->bpairs, B * 2 * ARGMAX_CTAS * (size_t)c.tp_size));
-    m->bcache_k.assign(c.n_layers, nullptr);
-    m->bcache_v.assign(c.n_layers, nullptr);
-    for (int l = 0; l < c.n_layers; ++l) {
-        LL_QMM(dev_alloc(m, &m->bcache_k[l], B * (size_t)m->kvl * c.max_seq * hd));
-        LL_QMM(dev_alloc(m, &m->bcache_v[l], B * (size_t)m->kvl * c.max_seq * hd));
+    if (paged) {
+        m->bwidth = (c.max_seq + page_tokens - 1) / page_tokens;
+        LL_QMM(dev_alloc(m, &m->btable, B * (size_t)m->bwidth));
+        LL_QMM(dev_alloc(m, &m->blen, B));
+        LL_QMM(dev_alloc(m, &m->prompt_rows, 3));
+        LL_QMM(dev_alloc(m, &m->bctx, B * ctx_w));
+        LL_QMM(dev_alloc(m, &m->bwork, QMM_KV_WORKSPACE_BYTES));
+        m->bpool.assign(c.n_layers, nullptr);
+        for (int l = 0; l < c.n_layers; ++l) {
+            LL_QMM(dev_alloc(m, &m->bpool[l], pool_bytes));
+        }
+        m->btable_host.assign(B * (size_t)m->bwidth, 0);
+        m->bheld.assign(batch, 0);
+        m->bfree.clear();
+        for (int64_t i = n_pages; i > 0; --i) {
+            m->bfree.push_back((int)(i - 1));
+        }
+    } else {
+        m->bcache_k.assign(c.n_layers, nullptr);
+        m->bcache_v.assign(c.n_layers, nullptr);
+        for (int l = 0; l < c.n_layers; ++l) {
+            LL_QMM(dev_alloc(m, &m->bcache_k[l], B * (size_t)m->kvl * c.max_seq * hd));
+            LL_QMM(dev_alloc(m, &m->bcache_v[l], B * (size_t)m->kvl * c.max_seq * hd));
+        }
     }
+    m->paged = paged;
     m->bpos_host.assign(batch, 0);
     m->btok_host.assign(batch, 0);
     m->bsteps_host = 0;
     m->batch_max_steps = max_steps;
     m->batch = batch;
+    return QMM_OK;
+}
+
+int qmm_llama_batch_create(qmm_llama* m, int batch, int max_steps)
+{
+    return batch_create(m, batch, max_steps, QMM_KV_F16, 0, 0);
+}
+
+int qmm_llama_batch_create_paged(qmm_llama* m, int batch, int max_steps, int kv_fmt, int page_tokens, int64_t n_pages)
+{
+    if (page_tokens == 0) {
+        return qmm_internal_fail(QMM_E_INVALID, "qmm_llama_batch_create_paged: a page holds at least 16 tokens");
+    }
+    return batch_create(m, batch, max_steps, kv_fmt, page_tokens, n_pages);
+}
+
+int qmm_llama_batch_free_pages(const qmm_llama* m, int64_t* free_pages)
+{
+    if (!m || !m->paged || !free_pages) {
+        return qmm_internal_fail(QMM_E_INVALID, "qmm_llama_batch_free_pages: no paged batch, or a null argument");
+    }
+    *free_pages = (int64_t)m->bfree.size();
     return QMM_OK;
 }
 
@@ -1138,8 +1309,17 @@ int qmm_llama_batch_prefill(qmm_llama* m, int seq, const int32_t* tokens_host, i
     // (position, token count, current token; the list entry the prefill appends lies beyond the count) is
     // put back afterwards, so batch and single sequence can be used side by side.
     const size_t stride = (size_t)m->kvl * m->cfg.max_seq * m->cfg.head_dim;
+    if (m->paged) {
+        if (!tokens_host || n < 1 || n > m->cfg.max_prefill || n > m->cfg.max_seq) {
+            return qmm_internal_fail(QMM_E_INVALID, "qmm_llama_batch_prefill: prompt length outside 1..max_prefill or cache full");
+        }
+        LL_GUARD(m);
+        std::vector<int> tokens(m->batch, 0);
+        tokens[seq] = n;
+        LL_QMM(reserve_pages(m, tokens, static_cast<cudaStream_t>(stream)));
+    }
     std::vector<std::pair<__half*, __half*>> own(m->layers.size());
-    for (size_t l = 0; l < m->layers.size(); ++l) {
+    for (size_t l = 0; l < m->layers.size() && !m->paged; ++l) {
         own[l] = {m->layers[l].cache_k, m->layers[l].cache_v};
         m->layers[l].cache_k = m->bcache_k[l] + (size_t)seq * stride;
         m->layers[l].cache_v = m->bcache_v[l] + (size_t)seq * stride;
@@ -1158,9 +1338,9 @@ int qmm_llama_batch_prefill(qmm_llama* m, int seq, const int32_t* tokens_host, i
     m->host_pos = 0;
     m->pick_with_nccl = true;
     int32_t first = 0;
-    const int rc = qmm_llama_prefill(m, tokens_host, n, &first, stream);
+    const int rc = prefill_rows(m, tokens_host, n, &first, m->paged ? seq : -1, stream);
     m->pick_with_nccl = false;
-    for (size_t l = 0; l < m->layers.size(); ++l) {
+    for (size_t l = 0; l < m->layers.size() && !m->paged; ++l) {
         m->layers[l].cache_k = own[l].first;
         m->layers[l].cache_v = own[l].second;
     }
@@ -1197,6 +1377,13 @@ int qmm_llama_batch_decode_enqueue(qmm_llama* m, int steps, void* stream)
     }
     LL_GUARD(m);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (m->paged && (st != nullptr || m->bgraph)) {
+        std::vector<int> tokens(m->bpos_host);
+        for (int& t : tokens) {
+            t += m->bsteps_host + steps;
+        }
+        LL_QMM(reserve_pages(m, tokens, st));
+    }
     if (!m->bgraph) {
         if (st == nullptr) {
             return qmm_internal_fail(QMM_E_INVALID, "qmm_llama_batch_decode needs a non-default stream (graph capture)");

@@ -217,6 +217,26 @@ __global__ void rope_table_kernel(int max_seq, int rope_dim, double theta, float
     }
 }
 
+__global__ void rope_table_from_kernel(int max_seq, int half, const double* __restrict__ inv_freq, double gain,
+                                       float* __restrict__ rope_cos, float* __restrict__ rope_sin)
+{
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < (int64_t)max_seq * half;
+         i += (int64_t)gridDim.x * blockDim.x) {
+        const double ang = (double)(i / half) * inv_freq[i % half];
+        rope_cos[i] = (float)(cos(ang) * gain);
+        rope_sin[i] = (float)(sin(ang) * gain);
+    }
+}
+
+__global__ void next_lengths_kernel(const int* __restrict__ pos, int batch, int* __restrict__ len)
+{
+    pdl_trigger();
+    pdl_sync();
+    if ((int)threadIdx.x < batch) {
+        len[threadIdx.x] = pos[threadIdx.x] + 1;
+    }
+}
+
 // RoPE on q and k of one token at position *pos, K/V appended to the fp16 cache.
 //   qkv: [n_heads*hd | n_kv*hd | n_kv*hd] fp32 (q rotated in place)
 //   cache_k / cache_v: [n_kv][max_seq][hd] fp16
@@ -1289,6 +1309,21 @@ cudaError_t ll_rope_tables(int max_seq, int rope_dim, double theta, float* rope_
 {
     rope_table_kernel<<<64, 256, 0, st>>>(max_seq, rope_dim, theta, rope_cos, rope_sin);
     return cudaGetLastError();
+}
+
+cudaError_t ll_rope_tables_from(int max_seq, int rope_dim, const double* inv_freq, double gain, float* rope_cos, float* rope_sin,
+                                cudaStream_t st)
+{
+    rope_table_from_kernel<<<64, 256, 0, st>>>(max_seq, rope_dim / 2, inv_freq, gain, rope_cos, rope_sin);
+    return cudaGetLastError();
+}
+
+cudaError_t ll_next_lengths(const int* pos, int batch, int* len, cudaStream_t st)
+{
+    if (batch < 1 || batch > 1024) {
+        return cudaErrorInvalidValue;
+    }
+    return launch_pdl(next_lengths_kernel, dim3(1), dim3((batch + 31) / 32 * 32), 0, st, pos, batch, len);
 }
 
 cudaError_t ll_embed_rows(int fmt, const uint8_t* raw, const int* tokens, int n_rows, int d, float* h, cudaStream_t st)

@@ -9,6 +9,11 @@
 namespace qmm {
 
 cudaError_t ll_rope_tables(int max_seq, int rope_dim, double theta, float* rope_cos, float* rope_sin, cudaStream_t st);
+// The same tables from given frequencies [rope_dim / 2] (device), the rotation times `gain`.
+cudaError_t ll_rope_tables_from(int max_seq, int rope_dim, const double* inv_freq, double gain, float* rope_cos, float* rope_sin,
+                                cudaStream_t st);
+// len[i] = pos[i] + 1 (batch <= 1024).
+cudaError_t ll_next_lengths(const int* pos, int batch, int* len, cudaStream_t st);
 cudaError_t ll_embed_rows(int fmt, const uint8_t* raw, const int* tokens, int n_rows, int d, float* h, cudaStream_t st);
 // Receiving side of the tensor-parallel sum that PeerScatter (qmm_common.cuh) feeds; tp_size <= 1 = off.
 struct PeerGather {

@@ -199,6 +199,31 @@ class LlamaModel:
         capi.check(capi.load().qmm_llama_batch_create(self._h, int(batch), int(max_steps)))
         self.batch = int(batch)
 
+    def batch_create_paged(self, batch: int, max_steps: int, kv_fmt: int = capi.Q4_0, page_tokens: int = 64,
+                           n_pages: int | None = None) -> None:
+        """A batch whose caches are pages of `kv_fmt` (capi.KV_F16, Q8_0, Q4_0) that the sequences share; `n_pages` defaults to
+        what max_seq positions of every sequence take."""
+        if n_pages is None:
+            n_pages = int(batch) * -(-self.spec.max_seq // max(1, int(page_tokens)))
+        capi.check(capi.load().qmm_llama_batch_create_paged(self._h, int(batch), int(max_steps), int(kv_fmt),
+                                                            int(page_tokens), int(n_pages)))
+        self.batch = int(batch)
+
+    def batch_free_pages(self) -> int:
+        out = ctypes.c_int64()
+        capi.check(capi.load().qmm_llama_batch_free_pages(self._h, ctypes.byref(out)))
+        return out.value
+
+    def set_rope_scaling(self, scaling: capi.RopeScaling | None = None, factors: np.ndarray | None = None) -> None:
+        """Rotary frequencies of a stretched context; `factors`: fp32 [rope_dim / 2] divisors (rope_freqs.weight)."""
+        if factors is not None:
+            factors = np.ascontiguousarray(factors, dtype=np.float32)
+            if factors.shape != (self.spec.rdim // 2,):
+                raise ValueError("one factor per pair of rotated dimensions is required")
+        capi.check(capi.load().qmm_llama_set_rope_scaling(
+            self._h, ctypes.c_void_p(None if factors is None else factors.ctypes.data),
+            None if scaling is None else ctypes.byref(scaling)))
+
     def batch_prefill(self, seq: int, tokens: np.ndarray) -> int:
         tokens = np.ascontiguousarray(tokens, dtype=np.int32)
         first = ctypes.c_int32()

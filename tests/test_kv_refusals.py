@@ -178,3 +178,11 @@ def test_null_structures():
     assert L.qmm_kv_append(0, cache().desc, None, None, 0, 0, None, 0, None, 0, None, 0, None, 0, 0, None) == capi.E_INVALID
     assert L.qmm_kv_read(0, None, None, None, 0, None, 0, 0, None) == capi.E_INVALID
     assert L.qmm_rope_frequencies(64, 1e4, None, None, None, None) == capi.E_INVALID
+
+
+def test_decoder_entry_points_without_a_model():
+    L = capi.load()
+    assert L.qmm_llama_set_rope_scaling(None, None, None) == capi.E_INVALID
+    assert L.qmm_llama_batch_create_paged(None, 1, 1, 1, 0, 1) == capi.E_INVALID
+    assert L.qmm_llama_batch_create_paged(None, 1, 1, 1, 64, 1) == capi.E_INVALID
+    assert L.qmm_llama_batch_free_pages(None, ctypes.byref(ctypes.c_int64())) == capi.E_INVALID
