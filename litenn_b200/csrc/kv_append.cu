@@ -54,47 +54,45 @@ __device__ __forceinline__ float2 turned(float x, float y, double2 cs)
 }
 
 // The eight lanes of a 32-dimension block hold four values each: the block's scale and this lane's four quants, by GGUF's
-// rules in fp32 (no contraction: the bytes must not depend on how the compiler joins a product and a sum).
+// rules in fp32 (no contraction: the bytes must not depend on how the compiler joins a product and a sum).  Magnitudes are
+// compared as their bits, which puts infinities and NaN above all else.
 template <int FMT>
 __device__ __forceinline__ float quantize4(const float (&x)[4], int lane, uint32_t (&q)[4])
 {
-    float top = x[0], size = fabsf(x[0]);
-    bool odd = !isfinite(x[0]);
+    float top = x[0];
+    uint32_t size = __float_as_uint(x[0]) & 0x7FFFFFFFu;
 #pragma unroll
     for (int i = 1; i < 4; ++i) {
-        odd |= !isfinite(x[i]);
-        if (fabsf(x[i]) > size) {  // the first of equals
-            size = fabsf(x[i]);
-            top = x[i];
-        }
+        const uint32_t bits = __float_as_uint(x[i]) & 0x7FFFFFFFu;
+        top = bits > size ? x[i] : top;  // the first of equals
+        size = max(size, bits);
     }
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) {
         const float other = __shfl_xor_sync(0xFFFFFFFFu, top, o);
+        const uint32_t bits = __float_as_uint(other) & 0x7FFFFFFFu;
         const bool lower = (lane & o) != 0;  // the other lane's values come first
-        if (fabsf(other) > size || (lower && fabsf(other) == size)) {
-            size = fabsf(other);
-            top = other;
-        }
+        top = bits > size || (lower && bits == size) ? other : top;
+        size = max(size, bits);
     }
-    const bool any_odd = (__ballot_sync(0xFFFFFFFFu, odd) >> (lane & 24) & 0xFFu) != 0;
-    float d = FMT == FMT_Q4_0 ? __fdiv_rn(top, -8.0f) : __fdiv_rn(size, 127.0f);
-    d = fminf(fmaxf(d, -65504.0f), 65504.0f);  // more than fp16 holds: the values saturate
-    const float inverse = d == 0.0f ? 0.0f : __fdiv_rn(1.0f, d);
+    const bool odd = size >= 0x7F800000u;
+    constexpr float MOST = FMT == FMT_Q4_0 ? 8188.0f : 515.5f;  // q * d stays within fp16's range
+    float d = FMT == FMT_Q4_0 ? top * -0.125f : __fdiv_rn(__uint_as_float(size), 127.0f);
+    d = fminf(fmaxf(d, -MOST), MOST);
+    const float inverse = d == 0.0f ? 0.0f : __frcp_rn(d);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+        // the whole part of a number from 0 to 2^23: the last bits of its sum with 2^23, rounded down (no conversion unit)
         const float y = __fmul_rn(x[i], inverse);
         if (FMT == FMT_Q4_0) {
-            q[i] = (uint32_t)fminf(fmaxf(floorf(__fadd_rn(y, 8.5f)), 0.0f), 15.0f);
+            q[i] = __float_as_uint(__fadd_rd(fminf(fmaxf(__fadd_rn(y, 8.5f), 0.0f), 15.0f), 8388608.0f)) & 15u;
         } else {
-            const float r = fminf(floorf(__fadd_rn(fabsf(y), 0.5f)), 127.0f);
-            q[i] = (uint32_t)(int)(copysignf(r, y) + 128.0f);
+            const uint32_t r = __float_as_uint(__fadd_rd(fminf(__fadd_rn(fabsf(y), 0.5f), 127.0f), 8388608.0f)) & 127u;
+            q[i] = y < 0.0f ? 128u - r : 128u + r;
         }
-        if (any_odd) {
-            q[i] = FMT == FMT_Q4_0 ? 8u : 128u;
-        }
+        q[i] = odd ? (FMT == FMT_Q4_0 ? 8u : 128u) : q[i];
     }
-    return any_odd ? __uint_as_float(0x7FC00000u) : d;
+    return odd ? __uint_as_float(0x7FC00000u) : d;
 }
 
 // Stores four consecutive values of a token: `keys` tells which plane's order.  All 32 lanes call it; `on` lanes store.
@@ -125,10 +123,12 @@ __device__ __forceinline__ void put4(uint8_t* tile, int hd, bool keys, int token
     uint32_t q[4];
     const float d = quantize4<FMT>(x, lane, q);
     if (FMT == FMT_Q4_0) {
-        if (keys) {  // dims 4h.. of a lane's eight: bytes h and h + 2 of its word, the pair of lanes joins them
-            const uint32_t h = (uint32_t)(dim >> 2) & 1u;
-            const uint32_t mine = ((q[0] | q[2] << 4) | (q[1] | q[3] << 4) << 16) << (8u * h);
-            const uint32_t word = mine | __shfl_xor_sync(0xFFFFFFFFu, mine, 1);
+        // keys: dims 4h.. of a lane's eight are bytes h and h + 2 of its word, the pair of lanes joins them.  All lanes take part:
+        // a warp may hold keys and values
+        const uint32_t h = (uint32_t)(dim >> 2) & 1u;
+        const uint32_t mine = ((q[0] | q[2] << 4) | (q[1] | q[3] << 4) << 16) << (8u * h);
+        const uint32_t word = mine | __shfl_xor_sync(0xFFFFFFFFu, mine, 1);
+        if (keys) {
             if (on && h == 0) {
                 *reinterpret_cast<uint32_t*>(tile + kv_place(FMT, hd, j, 4 * (token & 7) + (dim >> 3 & 3), b, 0)) = word;
             }
@@ -159,28 +159,47 @@ __device__ __forceinline__ void get4(const uint8_t* tile, int hd, bool keys, int
 {
     const int b = dim >> 5, first = keys ? 0 : kv_plane_bytes(FMT, hd) + kv_scale_bytes(FMT, hd);
     const int j = token >> 3, e = token & 1;
-    const uint8_t* at = keys ? tile + kv_place(FMT, hd, j, 4 * (token & 7) + (dim >> 3 & 3), b, 0)
-                             : tile + first + kv_place(FMT, hd, j, 4 * (dim >> 2 & 7) + (token >> 1 & 3), b, 0);
+    const int lane = keys ? 4 * (token & 7) + (dim >> 3 & 3) : 4 * (dim >> 2 & 7) + (token >> 1 & 3);
+    const uint8_t* at = tile + first + kv_place(FMT, hd, j, lane, b, 0);  // the lane's eight values of the block
+    const int half = dim >> 2 & 1;                                        // keys: which four of them
     if (FMT == KV_F16) {
-        const __half* h = reinterpret_cast<const __half*>(at);
+        if (keys) {
+            const uint2 w = *reinterpret_cast<const uint2*>(at + 8 * half);
+            const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), hi = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+            x[0] = lo.x, x[1] = lo.y, x[2] = hi.x, x[3] = hi.y;
+        } else {
+            const uint4 w = *reinterpret_cast<const uint4*>(at);  // pairs of tokens
+            const uint32_t v[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[i] = __half2float(h[keys ? (dim & 4) + i : 2 * i + e]);
+            for (int i = 0; i < 4; ++i) {
+                x[i] = __half2float(__ushort_as_half((unsigned short)(v[i] >> (16 * e))));
+            }
         }
         return;
     }
     const float d = __half2float(
         *reinterpret_cast<const __half*>(tile + first + kv_plane_bytes(FMT, hd) + kv_scale_place(hd, token, b)));
+    int q[4];
+    if (FMT == FMT_Q4_0) {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(at);
+        // keys: dimension 4 half + i is nibble 2 half + (i >> 1) of the lower (i even) or the upper 16 bits; values: nibble i of
+        // the token's 16 bits
+        const uint32_t lo = keys ? w >> (8 * half) : w >> (16 * e), hi = keys ? w >> (16 + 8 * half) : lo >> 8;
+        q[0] = (int)(lo & 15u);
+        q[1] = (int)(keys ? hi & 15u : lo >> 4 & 15u);
+        q[2] = (int)(keys ? lo >> 4 & 15u : hi & 15u);
+        q[3] = (int)(hi >> 4 & 15u);
+    } else {
+        const uint2 w = *reinterpret_cast<const uint2*>(at);
+        const uint32_t k = half ? w.y : w.x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            q[i] = (int)(keys ? k >> (8 * i) & 255u : (i < 2 ? w.x : w.y) >> (16 * (i & 1) + 8 * e) & 255u);
+        }
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        int q;
-        if (FMT == FMT_Q4_0) {
-            const int r = keys ? (dim >> 1 & 2) + (i >> 1) : i, second = keys ? i & 1 : e;
-            q = (at[(r >> 1) + 2 * second] >> (4 * (r & 1)) & 15) - 8;
-        } else {
-            q = (int)at[keys ? (dim & 4) + i : 2 * i + e] - 128;
-        }
-        x[i] = (float)q * d;
+        x[i] = (float)(q[i] - (FMT == FMT_Q4_0 ? 8 : 128)) * d;
     }
 }
 
@@ -337,6 +356,366 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvReadArgs a)
     }
 }
 
+// ---- prompts: one tile of 16 tokens per CTA and group of heads -----------------------------------------------------------
+// A token's values lie in pieces of 1 to 4 bytes all over a tile (two tokens share an operand register), so whole tiles are put
+// together in shared memory and leave as 16-byte stores; a sequence's first and last tile may be shared with tokens that are
+// there already and are stored piece by piece.  Bound: bytes (rows in, queries out, tiles out).
+
+// A tile of a call: 16 positions of a sequence, those from `begin` to `end` being rows of the call from `row` on.
+struct TilePlace {
+    int seq, pos0, begin, end;  // seq < 0: there is no such tile
+    int64_t row;
+};
+// The `want`-th tile over all sequences.  Whole CTA; reports what is bad.
+__device__ __forceinline__ TilePlace find_tile(const KvPool& c, const KvSeqs& b, int64_t want, TilePlace* shared)
+{
+    if (threadIdx.x < 32) {
+        const int lane = threadIdx.x;
+        TilePlace p = {-1, 0, 0, 0, 0};
+        int64_t before = 0;
+        for (int base = 0; base < b.batch && p.seq < 0 && before <= want; base += 32) {
+            const int s = base + lane;
+            bool bad = false;
+            KvSeq q = {0, 0, 0};
+            if (s < b.batch) {
+                q = kv_seq(c, b, s, bad);
+                bad = bad || q.len < q.n;
+            }
+            if (bad) {
+                q.n = 0;
+                if (want == 0) {
+                    atomicExch(b.status, KV_BAD_ROWS);
+                }
+            }
+            const int first = q.len - q.n, t0 = q.n > 0 ? first / KV_TILE : 0;
+            int64_t upto = q.n > 0 ? (q.len - 1) / KV_TILE - t0 + 1 : 0;
+            const int64_t mine = upto;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t u = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+                upto += lane >= o ? u : 0;
+            }
+            const bool here = mine > 0 && before + upto - mine <= want && want < before + upto;
+            if (here) {
+                const int tile = t0 + (int)(want - (before + upto - mine));
+                p.seq = s;
+                p.pos0 = tile * KV_TILE;
+                p.begin = max(0, first - p.pos0);
+                p.end = min(KV_TILE, q.len - p.pos0);
+                p.row = q.row0 + (p.pos0 + p.begin - first);
+                *shared = p;
+            }
+            p.seq = __any_sync(0xFFFFFFFFu, here) ? 0 : -1;
+            before += __shfl_sync(0xFFFFFFFFu, upto, 31);
+        }
+        if (p.seq < 0 && lane == 0) {
+            *shared = p;
+        }
+    }
+    __syncthreads();
+    return *shared;
+}
+// At most this many tiles hold rows of a call.
+int64_t tiles_of(const KvSeqs& b)
+{
+    return b.rows / KV_TILE + 2 * (int64_t)b.batch;
+}
+
+constexpr int TILE_Q_HEADS = 16;  // query heads of a CTA that has those
+template <int FMT, int HD>
+struct TileShape {
+    static constexpr int BYTES = kv_tile_bytes(FMT, HD);
+    static constexpr int KV_HEADS = BYTES <= 4608 ? 8 : BYTES <= 8192 ? 4 : 2;  // kv heads of a CTA that has those
+    static constexpr int LANES = HD / 4;                    // that a head's row takes, four values each
+    // A warp's lane keeps its dimensions from head to head, so it reads its angles once per row: LW lanes and SEGS turns to a
+    // head, HPW heads at once.
+    static constexpr int LW = LANES < 32 ? LANES : 32, SEGS = LANES / LW, HPW = 32 / LW;
+};
+
+// A lane's angles: of its pairs (dim, dim + 1), (dim + 2, dim + 3), or in halves of its four dimensions (either half's).
+template <bool HALVES>
+struct Angles {
+    double2 cs[HALVES ? 4 : 2];
+    __device__ __forceinline__ void load(const double2* turn, int dim, int n)
+    {
+        const int first = HALVES ? (dim >= n ? dim - n : dim) : dim >> 1;
+        if (dim < 2 * n) {
+#pragma unroll
+            for (int i = 0; i < (HALVES ? 4 : 2); ++i) {
+                cs[i] = HALVES || first + i < n ? turn[first + i] : make_double2(1.0, 0.0);
+            }
+        }
+    }
+};
+
+// blockIdx.x: groups of kv heads, then groups of query heads; blockIdx.y: tiles.
+template <int FMT, int HD, bool HALVES>
+__global__ void __launch_bounds__(256) kv_append_tile_kernel(const KvAppendArgs a)
+{
+    using Shape = TileShape<FMT, HD>;
+    constexpr int UNROLL = 4;
+    extern __shared__ __align__(16) uint8_t append_smem[];
+    __shared__ TilePlace place;
+    double2* turn = reinterpret_cast<double2*>(append_smem);  // [16][rope.dim / 2]
+    const int n = a.rope.dim / 2;
+    uint8_t* tiles = append_smem + (size_t)KV_TILE * n * sizeof(double2);  // [KV_HEADS]
+    pdl_trigger();
+    pdl_sync();
+    const TilePlace at = find_tile(a.pool, a.seqs, blockIdx.y, &place);
+    if (at.seq < 0) {
+        return;
+    }
+    const int rows = at.end - at.begin;
+    for (int i = threadIdx.x; i < rows * n; i += blockDim.x) {
+        double s, c;
+        sincos((double)(at.pos0 + at.begin + i / n) * a.rope.inv_freq[i % n], &s, &c);
+        turn[i] = make_double2(c * a.rope.gain, s * a.rope.gain);
+    }
+    __syncthreads();
+    const int kv_groups = (a.pool.kv_heads + Shape::KV_HEADS - 1) / Shape::KV_HEADS;
+    const int lane = threadIdx.x & 31;
+    if ((int)blockIdx.x >= kv_groups) {
+        // queries: every thread takes four dimensions of a head's row (in halves eight, so that they may be turned in place)
+        const int h0 = ((int)blockIdx.x - kv_groups) * TILE_Q_HEADS, heads = min(TILE_Q_HEADS, a.heads - h0);
+        for (int r = threadIdx.x >> 5; r < rows; r += 8) {
+            const int64_t in = (at.row + r) * a.q_stride + (int64_t)h0 * HD, out = (at.row + r) * a.q_out_stride + (int64_t)h0 * HD;
+#pragma unroll
+            for (int seg = 0; seg < Shape::SEGS; ++seg) {
+                const int dim = lane % Shape::LW * 4 + seg * 128;
+                const bool turns = dim < 2 * n, on = lane < Shape::HPW * Shape::LW && !(HALVES && turns && dim >= n);
+                Angles<HALVES> t;
+                t.load(turn + r * n, dim, n);
+                for (int base = lane / Shape::LW; base < heads; base += UNROLL * Shape::HPW) {
+                    float x[UNROLL][4], y[UNROLL][4];
+#pragma unroll
+                    for (int u = 0; u < UNROLL; ++u) {
+                        const int h = base + u * Shape::HPW;
+                        if (on && h < heads) {
+                            load4(a.q, in + h * HD + dim, a.type, x[u]);
+                            if (HALVES && turns) {
+                                load4(a.q, in + h * HD + dim + n, a.type, y[u]);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int u = 0; u < UNROLL; ++u) {
+                        const int h = base + u * Shape::HPW;
+                        if (!on || h >= heads) {
+                            continue;
+                        }
+                        if (turns) {
+#pragma unroll
+                            for (int i = 0; i < (HALVES ? 4 : 2); ++i) {
+                                if (HALVES) {
+                                    const float2 z = turned(x[u][i], y[u][i], t.cs[i]);
+                                    x[u][i] = z.x, y[u][i] = z.y;
+                                } else if (dim + 2 * i < 2 * n) {
+                                    const float2 z = turned(x[u][2 * i], x[u][2 * i + 1], t.cs[i % 2]);
+                                    x[u][2 * i % 4] = z.x, x[u][(2 * i + 1) % 4] = z.y;
+                                }
+                            }
+                            if (HALVES) {
+                                store4(a.q_out, out + h * HD + dim + n, a.q_type, y[u]);
+                            }
+                        }
+                        store4(a.q_out, out + h * HD + dim, a.q_type, x[u]);
+                    }
+                }
+            }
+        }
+        return;
+    }
+    const int h0 = (int)blockIdx.x * Shape::KV_HEADS, heads = min(Shape::KV_HEADS, a.pool.kv_heads - h0);
+    const int page = kv_page(a.pool, a.seqs, at.seq, at.pos0);
+    if (page < 0) {
+        if (threadIdx.x == 0) {
+            atomicExch(a.seqs.status, KV_BAD_PAGE);
+        }
+        return;
+    }
+    const bool whole = rows == KV_TILE;
+    for (int r = threadIdx.x >> 5; r < rows; r += 8) {
+#pragma unroll
+        for (int seg = 0; seg < Shape::SEGS; ++seg) {
+            const int dim = lane % Shape::LW * 4 + seg * 128;
+            const bool turns = dim < 2 * n, on = lane < Shape::HPW * Shape::LW;
+            Angles<HALVES> t;
+            t.load(turn + r * n, dim, n);
+            // keys, then values; all lanes of a warp together: a block's eight take part in its maximum
+            for (int base = 0; base < 2 * heads; base += UNROLL * Shape::HPW) {
+                float x[UNROLL][4], y[UNROLL][4];
+#pragma unroll
+                for (int u = 0; u < UNROLL; ++u) {
+                    const int h = base + u * Shape::HPW + lane / Shape::LW;
+                    x[u][0] = x[u][1] = x[u][2] = x[u][3] = 0.0f;
+                    if (on && h < heads) {
+                        const int64_t in = (at.row + r) * a.k_stride + (int64_t)(h0 + h) * HD + dim;
+                        load4(a.k, in, a.type, x[u]);
+                        if (HALVES && turns) {
+                            load4(a.k, dim >= n ? in - n : in + n, a.type, y[u]);
+                        }
+                    } else if (on && h < 2 * heads) {
+                        load4(a.v, (at.row + r) * a.v_stride + (int64_t)(h0 + h - heads) * HD + dim, a.type, x[u]);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < UNROLL; ++u) {
+                    const int h = base + u * Shape::HPW + lane / Shape::LW;
+                    const bool keys = h < heads;
+                    if (keys && on && turns) {
+#pragma unroll
+                        for (int i = 0; i < (HALVES ? 4 : 2); ++i) {
+                            if (HALVES) {
+                                x[u][i] = dim >= n ? turned(y[u][i], x[u][i], t.cs[i]).y : turned(x[u][i], y[u][i], t.cs[i]).x;
+                            } else if (dim + 2 * i < 2 * n) {
+                                const float2 z = turned(x[u][2 * i], x[u][2 * i + 1], t.cs[i % 2]);
+                                x[u][2 * i % 4] = z.x, x[u][(2 * i + 1) % 4] = z.y;
+                            }
+                        }
+                    }
+                    const int mine = min(keys ? h : h - heads, heads - 1);
+                    uint8_t* tile = whole ? tiles + mine * Shape::BYTES
+                                          : a.pool.base + kv_tile_index(a.pool, page, h0 + mine, at.pos0) * Shape::BYTES;
+                    put4<FMT>(tile, HD, keys, at.begin + r, dim, x[u], lane, on && h < 2 * heads);
+                }
+            }
+        }
+    }
+    if (whole) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < heads * (Shape::BYTES / 16); i += blockDim.x) {
+            const int h = i / (Shape::BYTES / 16), k = i % (Shape::BYTES / 16);
+            reinterpret_cast<uint4*>(a.pool.base + kv_tile_index(a.pool, page, h0 + h, at.pos0) * Shape::BYTES)[k] =
+                reinterpret_cast<const uint4*>(tiles + h * Shape::BYTES)[k];
+        }
+    }
+}
+
+template <int FMT, int HD>
+__global__ void __launch_bounds__(256) kv_read_tile_kernel(const KvReadArgs a)
+{
+    using Shape = TileShape<FMT, HD>;
+    extern __shared__ __align__(16) uint8_t read_smem[];
+    __shared__ TilePlace place;
+    pdl_trigger();
+    pdl_sync();
+    const TilePlace at = find_tile(a.pool, a.seqs, blockIdx.y, &place);
+    if (at.seq < 0) {
+        return;
+    }
+    const int page = kv_page(a.pool, a.seqs, at.seq, at.pos0);
+    if (page < 0) {
+        if (threadIdx.x == 0) {
+            atomicExch(a.seqs.status, KV_BAD_PAGE);
+        }
+        return;
+    }
+    const int h0 = (int)blockIdx.x * Shape::KV_HEADS, heads = min(Shape::KV_HEADS, a.pool.kv_heads - h0);
+    for (int i = threadIdx.x; i < heads * (Shape::BYTES / 16); i += blockDim.x) {
+        const int h = i / (Shape::BYTES / 16), k = i % (Shape::BYTES / 16);
+        reinterpret_cast<uint4*>(read_smem + h * Shape::BYTES)[k] =
+            reinterpret_cast<const uint4*>(a.pool.base + kv_tile_index(a.pool, page, h0 + h, at.pos0) * Shape::BYTES)[k];
+    }
+    __syncthreads();
+    const int rows = at.end - at.begin;
+    const int lane = threadIdx.x & 31;
+    for (int r = threadIdx.x >> 5; r < rows; r += 8) {
+#pragma unroll
+        for (int seg = 0; seg < Shape::SEGS; ++seg) {
+            const int dim = lane % Shape::LW * 4 + seg * 128;
+            if (lane >= Shape::HPW * Shape::LW) {
+                continue;
+            }
+#pragma unroll 4
+            for (int h = lane / Shape::LW; h < 2 * heads; h += Shape::HPW) {
+                const bool keys = h < heads;
+                const int mine = keys ? h : h - heads;
+                float x[4];
+                get4<FMT>(read_smem + mine * Shape::BYTES, HD, keys, at.begin + r, dim, x);
+                store4(keys ? a.k : a.v, (at.row + r) * (keys ? a.k_stride : a.v_stride) + (int64_t)(h0 + mine) * HD + dim, a.type, x);
+            }
+        }
+    }
+}
+
+template <typename Args>
+cudaError_t launch_tiles(void (*kernel)(Args), const Args& a, int groups, int64_t tiles, size_t smem, bool (&configured)[64],
+                         size_t most_smem, cudaStream_t stream)
+{
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) {
+        return e;
+    }
+    if (device < 0 || device >= 64 || !configured[device]) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most_smem);
+        if (e != cudaSuccess) {
+            return e;
+        }
+        if (device >= 0 && device < 64) {
+            configured[device] = true;
+        }
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)groups, (unsigned)tiles);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
+template <int FMT, int HD, bool HALVES>
+cudaError_t append_tiles(const KvAppendArgs& a, cudaStream_t stream)
+{
+    using Shape = TileShape<FMT, HD>;
+    static bool configured[64] = {};
+    const int groups = (a.pool.kv_heads + Shape::KV_HEADS - 1) / Shape::KV_HEADS + (a.heads + TILE_Q_HEADS - 1) / TILE_Q_HEADS;
+    constexpr size_t TILES = (size_t)Shape::KV_HEADS * Shape::BYTES;
+    return launch_tiles(kv_append_tile_kernel<FMT, HD, HALVES>, a, groups, tiles_of(a.seqs),
+                        (size_t)KV_TILE * (a.rope.dim / 2) * sizeof(double2) + TILES, configured,
+                        (size_t)KV_TILE * (HD / 2) * sizeof(double2) + TILES, stream);
+}
+template <int FMT, int HD>
+cudaError_t read_tiles(const KvReadArgs& a, cudaStream_t stream)
+{
+    using Shape = TileShape<FMT, HD>;
+    static bool configured[64] = {};
+    constexpr size_t TILES = (size_t)Shape::KV_HEADS * Shape::BYTES;
+    return launch_tiles(kv_read_tile_kernel<FMT, HD>, a, (a.pool.kv_heads + Shape::KV_HEADS - 1) / Shape::KV_HEADS, tiles_of(a.seqs),
+                        TILES, configured, TILES, stream);
+}
+template <int FMT>
+cudaError_t append_tiles_fmt(const KvAppendArgs& a, cudaStream_t stream)
+{
+    const bool halves = a.rope.halves;
+    switch (a.pool.head_dim) {
+    case 64: return halves ? append_tiles<FMT, 64, true>(a, stream) : append_tiles<FMT, 64, false>(a, stream);
+    case 96: return halves ? append_tiles<FMT, 96, true>(a, stream) : append_tiles<FMT, 96, false>(a, stream);
+    case 128: return halves ? append_tiles<FMT, 128, true>(a, stream) : append_tiles<FMT, 128, false>(a, stream);
+    default: return halves ? append_tiles<FMT, 256, true>(a, stream) : append_tiles<FMT, 256, false>(a, stream);
+    }
+}
+template <int FMT>
+cudaError_t read_tiles_fmt(const KvReadArgs& a, cudaStream_t stream)
+{
+    switch (a.pool.head_dim) {
+    case 64: return read_tiles<FMT, 64>(a, stream);
+    case 96: return read_tiles<FMT, 96>(a, stream);
+    case 128: return read_tiles<FMT, 128>(a, stream);
+    default: return read_tiles<FMT, 256>(a, stream);
+    }
+}
+// Whether a call goes by tiles: sequences of half a tile and more on average, and no more tiles than a grid has.
+bool by_tiles(const KvSeqs& b)
+{
+    return b.rows >= (int64_t)8 * b.batch && tiles_of(b) <= 65535;
+}
+
 template <typename Args>
 cudaError_t launch_rows(void (*kernel)(Args), const Args& a, int64_t rows, int items, cudaStream_t stream)
 {
@@ -359,6 +738,11 @@ cudaError_t launch_rows(void (*kernel)(Args), const Args& a, int64_t rows, int i
 cudaError_t launch_kv_append(const KvAppendArgs& a, cudaStream_t stream)
 {
     const int items = (a.heads + 2 * a.pool.kv_heads) * a.pool.head_dim / 4;
+    if (by_tiles(a.seqs)) {
+        return a.pool.fmt == FMT_Q4_0   ? append_tiles_fmt<FMT_Q4_0>(a, stream)
+               : a.pool.fmt == FMT_Q8_0 ? append_tiles_fmt<FMT_Q8_0>(a, stream)
+                                        : append_tiles_fmt<KV_F16>(a, stream);
+    }
     switch (a.pool.fmt) {
     case FMT_Q4_0: return launch_rows(kv_append_kernel<FMT_Q4_0>, a, a.seqs.rows, items, stream);
     case FMT_Q8_0: return launch_rows(kv_append_kernel<FMT_Q8_0>, a, a.seqs.rows, items, stream);
@@ -369,6 +753,11 @@ cudaError_t launch_kv_append(const KvAppendArgs& a, cudaStream_t stream)
 cudaError_t launch_kv_read(const KvReadArgs& a, cudaStream_t stream)
 {
     const int items = 2 * a.pool.kv_heads * a.pool.head_dim / 4;
+    if (by_tiles(a.seqs)) {
+        return a.pool.fmt == FMT_Q4_0   ? read_tiles_fmt<FMT_Q4_0>(a, stream)
+               : a.pool.fmt == FMT_Q8_0 ? read_tiles_fmt<FMT_Q8_0>(a, stream)
+                                        : read_tiles_fmt<KV_F16>(a, stream);
+    }
     switch (a.pool.fmt) {
     case FMT_Q4_0: return launch_rows(kv_read_kernel<FMT_Q4_0>, a, a.seqs.rows, items, stream);
     case FMT_Q8_0: return launch_rows(kv_read_kernel<FMT_Q8_0>, a, a.seqs.rows, items, stream);

@@ -35,7 +35,8 @@ def codes(x, fmt):
         first = np.argmax(np.where(np.isnan(size), -1, size), -1)[..., None]  # numpy takes the lowest index of equals
         top = np.take_along_axis(blk, first, -1)
         d = top / np.float32(-8) if fmt == Q4_0 else np.abs(top) / np.float32(127)
-        d = np.clip(d, np.float32(-65504), np.float32(65504)).astype(np.float32)
+        most = np.float32(8188) if fmt == Q4_0 else np.float32(515.5)  # values within fp16's range
+        d = np.clip(d, -most, most).astype(np.float32)
         inv = np.where(d == 0, np.float32(0), np.float32(1) / d)
         y = blk * inv
         if fmt == Q4_0:
