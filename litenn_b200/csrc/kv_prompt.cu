@@ -895,11 +895,14 @@ cudaError_t launch_prompt_fmt(const KvAttnArgs& a, int sm_count, cudaStream_t st
 
 }  // namespace
 
-// bf16 results of sequences that fill half an M tile on average.
+// bf16 results of enough columns: a list item (256 columns of a kv head) is one CTA's, from its first key to its last, where the
+// rows kernel cuts anything over the whole GPU.  2000 tokens of 128 dimensions, rows / prompt kernel, Q4_0: one sequence of 32 rows
+// of 64 heads 43 / 56 us, of 64 rows 69 / 56 us; of 64 rows of 32 heads (one to a kv head) 43 / 49 us, of 128 rows 68 / 51 us; eight
+// sequences of 4 rows of 64 heads 44 / 49 us, of 8 rows 69 / 49 us, of 16 rows of 32 heads (16 columns each) 70 / 102 us.
 bool kv_takes_prompt(const KvAttnArgs& a)
 {
     return a.out_type == QMM_OUT_BF16 && (a.pool.head_dim == 64 || a.pool.head_dim == 128) && a.seqs.row_begin != nullptr &&
-           a.seqs.rows * a.group >= (int64_t)64 * a.seqs.batch;
+           a.seqs.rows * a.group >= (int64_t)64 * a.seqs.batch && a.seqs.rows * a.group * a.pool.kv_heads >= 4096;
 }
 
 cudaError_t launch_kv_prompt(const KvAttnArgs& a, int sm_count, cudaStream_t stream)

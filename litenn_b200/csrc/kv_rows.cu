@@ -191,9 +191,11 @@ struct RowsShape {
     static constexpr int COLS = 8 * NT;  // columns of a pass
     static constexpr int TILE = kv_tile_bytes(FMT, HD);
     static constexpr int WARPS = 4;
-    // Tiles of a step.  Two halve what a step costs beside its products; where the sums take 64 registers, or two
-    // tiles of every warp a third of the SM, one leaves room for more CTAs.
-    static constexpr int STEP = NT * HD <= 128 && TILE <= 4608 ? 2 : 1;
+    // Tiles of a step.  Two halve what a step costs beside its products (one token, Q4_0, one / two: 131072 tokens of 8 kv heads of
+    // 128 63.4 / 60.8 us, of 96 60.0 / 50.0 us, 8 drafts of 2000 tokens Q8_0 22.1 / 19.9 us; 64 sequences of 1000 tokens, whose warps
+    // have a handful each, 45.3 / 49.3 us).  Where the sums take 64 registers one leaves room for more CTAs (16 columns of 64, 8
+    // sequences of 2000 tokens, 26.6 / 31.8 us), and fp16 has no scales to share (64 dimensions, 131072 tokens 52.8 / 57.4 us).
+    static constexpr int STEP = NT == 1 && HD <= 128 && FMT != KV_F16 ? 2 : 1;
     // CTAs per SM, by the registers the sums take (NT * HD / 4 of them)
     static constexpr int BY_REGISTERS = NT * HD <= 128 ? 4 : NT * HD <= 256 ? 3 : 1;
     static constexpr int DEPTH = 2;  // steps in the ring; three were no faster (131072 tokens, 64/8 heads, Q4_0: 62.8 us, two 60.9)
@@ -487,7 +489,7 @@ __global__ void __launch_bounds__(RowsShape<FMT, HD, NT>::WARPS * 32, RowsShape<
         constexpr int BP = VB % 2 == 0 ? 2 : 1;                                                                 // and those multiplied in turn
 
         for (int i = 0; i < my_steps; ++i) {
-            const int slot = i % DEPTH, tok0 = (tile_begin + (warp + i * WARPS) * STEP) * KV_TILE;
+            const int slot = i % DEPTH, step_tok0 = (tile_begin + (warp + i * WARPS) * STEP) * KV_TILE;
             if ((i & (AHEAD - 1)) == 0 && i > 0) {
                 place = place_next;
                 have_all = have_next;
@@ -502,15 +504,18 @@ __global__ void __launch_bounds__(RowsShape<FMT, HD, NT>::WARPS * 32, RowsShape<
                     atomicExch(a.seqs.status, KV_LATE_COPY);
                 }
             }
-            const uint8_t* base = my_ring + slot * STEP * TILE;
-            // two copies of what a step does: boundary tiles, where columns differ in what they see, pay for masks
-            auto multiply = [&](auto whole) {
+            // Two copies of what is done: whole steps, and single tiles, which pay for masks: those where columns differ in what
+            // they see, and a last one that has no second.
+            auto multiply = [&](auto whole, int first) {
                 constexpr bool WHOLE = decltype(whole)::value;
+                constexpr int N = WHOLE ? STEP : 1;
+                const uint8_t* base = my_ring + (slot * STEP + first) * TILE;
+                const int tok0 = step_tok0 + first * KV_TILE;
 
                 // ---- scores: s[n][j] of token tok0 + 8 j + g and columns 2t, 2t + 1 ----
-                float2 s[NT][2 * STEP];
+                float2 s[NT][2 * N];
 #pragma unroll
-                for (int u = 0; u < STEP; ++u) {
+                for (int u = 0; u < N; ++u) {
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         s[n][2 * u] = s[n][2 * u + 1] = make_float2(0.0f, 0.0f);
@@ -518,23 +523,23 @@ __global__ void __launch_bounds__(RowsShape<FMT, HD, NT>::WARPS * 32, RowsShape<
                 }
 #pragma unroll
                 for (int vb = 0; vb < NB / VB; ++vb) {
-                    uint32_t w[2 * STEP][VEC / 4];
+                    uint32_t w[2 * N][VEC / 4];
 #pragma unroll
-                    for (int j = 0; j < 2 * STEP; ++j) {
+                    for (int j = 0; j < 2 * N; ++j) {
                         load_words<VEC>(w[j], base + (j >> 1) * TILE + (j & 1) * 32 * LANE + vb * 32 * VEC + lane * VEC);
                     }
 #pragma unroll
                     for (int b0 = 0; b0 < VB; b0 += BP) {
-                        // BP * STEP * NT chains of four MMAs, in turn: an MMA's sum is ready for the next after about four others
-                        float c[BP][NT][STEP][4];
+                        // BP * N * NT chains of four MMAs, in turn: an MMA's sum is ready for the next after about four others
+                        float c[BP][NT][N][4];
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            uint32_t k[BP][STEP][4];
+                            uint32_t k[BP][N][4];
                             uint4 q[BP][NT];
 #pragma unroll
                             for (int bb = 0; bb < BP; ++bb) {
 #pragma unroll
-                                for (int u = 0; u < STEP; ++u) {
+                                for (int u = 0; u < N; ++u) {
                                     const uint32_t *w0 = w[2 * u] + (b0 + bb) * (U / 4), *w1 = w[2 * u + 1] + (b0 + bb) * (U / 4);
                                     k[bb][u][0] = key_operand<FMT>(w0, 2 * h);
                                     k[bb][u][1] = key_operand<FMT>(w1, 2 * h);
@@ -554,7 +559,7 @@ __global__ void __launch_bounds__(RowsShape<FMT, HD, NT>::WARPS * 32, RowsShape<
 #pragma unroll
                                     for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                                        for (int u = 0; u < STEP; ++u) {
+                                        for (int u = 0; u < N; ++u) {
                                             const uint32_t (&x)[4] = k[bb][u];
                                             const uint32_t q0 = part ? q[bb][n].y : q[bb][n].x, q1 = part ? q[bb][n].w : q[bb][n].z;
                                             if (h == 0 && part == 0) {
@@ -571,7 +576,7 @@ __global__ void __launch_bounds__(RowsShape<FMT, HD, NT>::WARPS * 32, RowsShape<
                         for (int bb = 0; bb < BP; ++bb) {
                             const int b = vb * VB + b0 + bb;
 #pragma unroll
-                            for (int u = 0; u < STEP; ++u) {
+                            for (int u = 0; u < N; ++u) {
 #pragma unroll
                                 for (int j = 0; j < 2; ++j) {
                                     const float d = QUANT ? __half2float(*reinterpret_cast<const __half*>(
@@ -590,13 +595,12 @@ __global__ void __launch_bounds__(RowsShape<FMT, HD, NT>::WARPS * 32, RowsShape<
                 }
                 if (!WHOLE) {
 #pragma unroll
-                    for (int j = 0; j < 2 * STEP; ++j) {
+                    for (int j = 0; j < 2 * N; ++j) {
                         const int pos = tok0 + 8 * j + g;
-                        const bool here = have >> (j >> 1) & 1u;
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            s[n][j].x = here && pos <= pos_of[n][0] && pos >= pos_of[n][0] - reach ? s[n][j].x : -INFINITY;
-                            s[n][j].y = here && pos <= pos_of[n][1] && pos >= pos_of[n][1] - reach ? s[n][j].y : -INFINITY;
+                            s[n][j].x = pos <= pos_of[n][0] && pos >= pos_of[n][0] - reach ? s[n][j].x : -INFINITY;
+                            s[n][j].y = pos <= pos_of[n][1] && pos >= pos_of[n][1] - reach ? s[n][j].y : -INFINITY;
                         }
                     }
                 }
@@ -606,7 +610,7 @@ __global__ void __launch_bounds__(RowsShape<FMT, HD, NT>::WARPS * 32, RowsShape<
                 for (int n = 0; n < NT; ++n) {
                     float2 top = s[n][0];
 #pragma unroll
-                    for (int j = 1; j < 2 * STEP; ++j) {
+                    for (int j = 1; j < 2 * N; ++j) {
                         top.x = fmaxf(top.x, s[n][j].x);
                         top.y = fmaxf(top.y, s[n][j].y);
                     }
@@ -635,30 +639,28 @@ __global__ void __launch_bounds__(RowsShape<FMT, HD, NT>::WARPS * 32, RowsShape<
                     }
                     const float2 ref = make_float2(m[n].x == -INFINITY ? 0.0f : -m[n].x, m[n].y == -INFINITY ? 0.0f : -m[n].y);
 #pragma unroll
-                    for (int j = 0; j < 2 * STEP; ++j) {  // s becomes the probabilities
+                    for (int j = 0; j < 2 * N; ++j) {  // s becomes the probabilities
                         const float2 x2 = fma2(s[n][j], qs[n], ref);
                         s[n][j] = make_float2(exp2_fast(x2.x), exp2_fast(x2.y));
                     }
                     if (!WHOLE) {
 #pragma unroll
-                        for (int j = 0; j < 2 * STEP; ++j) {  // also where qs is 0, or keys that are not there are NaN
+                        for (int j = 0; j < 2 * N; ++j) {  // also where qs is 0
                             const int pos = tok0 + 8 * j + g;
-                            const bool here = have >> (j >> 1) & 1u;
-                            s[n][j].x = here && pos <= pos_of[n][0] && pos >= pos_of[n][0] - reach ? s[n][j].x : 0.0f;
-                            s[n][j].y = here && pos <= pos_of[n][1] && pos >= pos_of[n][1] - reach ? s[n][j].y : 0.0f;
+                            s[n][j].x = pos <= pos_of[n][0] && pos >= pos_of[n][0] - reach ? s[n][j].x : 0.0f;
+                            s[n][j].y = pos <= pos_of[n][1] && pos >= pos_of[n][1] - reach ? s[n][j].y : 0.0f;
                         }
                     }
 #pragma unroll
-                    for (int j = 0; j < 2 * STEP; ++j) {
+                    for (int j = 0; j < 2 * N; ++j) {
                         l[n] = add2(l[n], s[n][j]);
                     }
                 }
 
                 // ---- values ----
 #pragma unroll
-                for (int u = 0; u < STEP; ++u) {
+                for (int u = 0; u < N; ++u) {
                     const uint8_t* vbase = base + u * TILE + PLANE + SCALES;
-                    const bool here = have >> u & 1u;
                     uint32_t all_see[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};  // tokens that every column sees (fp16 caches)
                     uint32_t keep[NT][2];                              // tokens that column g sees (quants)
                     uint32_t d[QUANT ? 2 * NB : 1];                    // value scales of tokens 2t, 2t + 1
@@ -677,8 +679,8 @@ __global__ void __launch_bounds__(RowsShape<FMT, HD, NT>::WARPS * 32, RowsShape<
                                 const int pos = tok0 + 16 * u + 8 * j + 2 * t;
 #pragma unroll
                                 for (int n = 0; n < NT; ++n) {
-                                    keep[n][j] = (here && pos <= op_pos[n] && pos >= op_pos[n] - reach ? 0x0000FFFFu : 0u) |
-                                                 (here && pos + 1 <= op_pos[n] && pos + 1 >= op_pos[n] - reach ? 0xFFFF0000u : 0u);
+                                    keep[n][j] = (pos <= op_pos[n] && pos >= op_pos[n] - reach ? 0x0000FFFFu : 0u) |
+                                                 (pos + 1 <= op_pos[n] && pos + 1 >= op_pos[n] - reach ? 0xFFFF0000u : 0u);
                                     any[j] |= keep[n][j];
                                 }
                             }
@@ -729,10 +731,10 @@ __global__ void __launch_bounds__(RowsShape<FMT, HD, NT>::WARPS * 32, RowsShape<
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
                             const int pos = tok0 + 16 * u + 8 * j + 2 * t;
-                            all_see[j] = (here && pos <= pos_lo && pos >= all_lo ? 0x0000FFFFu : 0u) |
-                                         (here && pos + 1 <= pos_lo && pos + 1 >= all_lo ? 0xFFFF0000u : 0u);
+                            all_see[j] = (pos <= pos_lo && pos >= all_lo ? 0x0000FFFFu : 0u) |
+                                         (pos + 1 <= pos_lo && pos + 1 >= all_lo ? 0xFFFF0000u : 0u);
                         }
-                        for (int tok = 0; tok < (here ? KV_TILE : 0); ++tok) {
+                        for (int tok = 0; tok < KV_TILE; ++tok) {
                             const int pos = tok0 + 16 * u + tok;
                             if ((pos <= pos_lo && pos >= all_lo) || pos > pos_hi || pos < seen_lo) {
                                 continue;
@@ -832,10 +834,15 @@ __global__ void __launch_bounds__(RowsShape<FMT, HD, NT>::WARPS * 32, RowsShape<
                 }
             };
             if (have != 0 && !late) {
-                if (have == (1u << STEP) - 1 && tok0 >= all_lo && tok0 + STEP * KV_TILE - 1 <= pos_lo) {
-                    multiply(std::true_type{});
+                if (have == (1u << STEP) - 1 && step_tok0 >= all_lo && step_tok0 + STEP * KV_TILE - 1 <= pos_lo) {
+                    multiply(std::true_type{}, 0);
                 } else {
-                    multiply(std::false_type{});
+#pragma unroll 1
+                    for (int u = 0; u < STEP; ++u) {
+                        if (have >> u & 1u) {
+                            multiply(std::false_type{}, u);
+                        }
+                    }
                 }
             }
             __syncwarp();
@@ -1053,13 +1060,16 @@ cudaError_t launch_rows(const KvAttnArgs& a, int sm_count, cudaStream_t stream)
 template <int FMT>
 cudaError_t launch_rows_fmt(const KvAttnArgs& a, int sm_count, cudaStream_t stream)
 {
-    // sixteen columns to a pass where a sequence may have more than eight
-    const bool wide = a.group > 8 || a.seqs.row_begin != nullptr;
+    // Sixteen columns to a pass where sequences have many, else eight: those leave registers for four CTAs an SM instead of three,
+    // which carries even two passes over the same keys.  8 sequences of 2000 tokens of 8 kv heads of 128, eight / sixteen: Q4_0 with 8
+    // columns each 24.7 / 30.0 us, 16 28.0 / 30.8 us, 32 43.5 / 41.0 us, 64 69.2 / 62.6 us; Q8_0 with 16 25.5 / 30.0 us, 64 62.9 / 62.2 us.
+    // At 256 dimensions sixteen leave one CTA and take twice eight's time (16 sequences of 2000 tokens, Q4_0, 92 and 42 us).
+    const bool wide = a.seqs.rows * a.group >= (int64_t)32 * a.seqs.batch;
     switch (a.pool.head_dim) {
     case 64: return wide ? launch_rows<FMT, 64, 2>(a, sm_count, stream) : launch_rows<FMT, 64, 1>(a, sm_count, stream);
     case 96: return wide ? launch_rows<FMT, 96, 2>(a, sm_count, stream) : launch_rows<FMT, 96, 1>(a, sm_count, stream);
     case 128: return wide ? launch_rows<FMT, 128, 2>(a, sm_count, stream) : launch_rows<FMT, 128, 1>(a, sm_count, stream);
-    case 256: return wide ? launch_rows<FMT, 256, 2>(a, sm_count, stream) : launch_rows<FMT, 256, 1>(a, sm_count, stream);
+    case 256: return launch_rows<FMT, 256, 1>(a, sm_count, stream);
     default: return cudaErrorInvalidValue;
     }
 }

@@ -79,15 +79,21 @@ class Paged:
         cut = np.cumsum(rows)[:-1]
         return np.split(ref.stored(k, self.fmt), cut), np.split(ref.stored(v, self.fmt), cut)
 
-    def attend(self, q, rows, lens, heads, bf16=False, out_bf16=False, window=0, single=False, scale=None, total=None):
+    def attend(self, q, rows, lens, heads, bf16=False, out_bf16=False, window=0, single=False, scale=None, total=None,
+               prompt=False):
         import torch
+        asked = len(q)
+        if prompt:  # rows behind the last sequence, so that the call is one of many
+            total = max(len(q), -(-4096 // heads))
+            q = np.concatenate([q, np.ones((total - len(q), *q.shape[1:]), q.dtype)])
         qd = torch_of(q.reshape(len(q), -1), bf16)
         out = torch.full((len(q), heads * self.hd), 7.0, device="cuda", dtype=torch.bfloat16 if out_bf16 else torch.float32)
         self.cache.attend(self.batch(rows, lens, total, single), heads, qd.data_ptr(), int(bf16), heads * self.hd,
                           out.data_ptr(), int(out_bf16), heads * self.hd, self.hd ** -0.5 if scale is None else scale, window,
                           self.workspace.data_ptr())
         assert capi.kernel_status(0) == 0
-        return np_of(out).reshape(len(q), heads, self.hd).astype(np.float64)
+        assert (out[asked:] == 7.0).all()
+        return np_of(out)[:asked].reshape(asked, heads, self.hd).astype(np.float64)
 
 
 def check_attention(p, rows, lens, heads, rng, bf16=False, out_bf16=False, window=0, single=False, q_scale=2.0, half=False):
@@ -109,15 +115,9 @@ def check_attention(p, rows, lens, heads, rng, bf16=False, out_bf16=False, windo
 
 # ---- append and read ----------------------------------------------------------------------------------------------------
 
-@pytest.mark.parametrize("fmt", FMTS)
-@pytest.mark.parametrize("hd,heads,kv_heads,page,rope_dim,halves,bf16", [
-    (128, 8, 2, 16, 128, False, False), (128, 4, 4, 64, 64, True, True), (64, 3, 1, 32, 64, True, False),
-    (96, 6, 3, 48, 96, True, False), (96, 2, 1, 16, 34, False, True), (256, 2, 2, 128, 256, True, False),
-    (256, 4, 1, 16, 0, False, False), (64, 2, 2, 16, 8, True, True)])
-def test_append_stores_what_the_rules_say(fmt, hd, heads, kv_heads, page, rope_dim, halves, bf16):
+def check_append(fmt, hd, heads, kv_heads, page, rope_dim, halves, bf16, rows, lens):
     import torch
     rng = np.random.default_rng(hd + page)
-    rows, lens = [5, 0, 1, 40], [21, 7, 1, 140]
     p = Paged(fmt, kv_heads, hd, page, lens)
     before = p.pool.clone()
     width = heads + 2 * kv_heads
@@ -152,7 +152,7 @@ def test_append_stores_what_the_rules_say(fmt, hd, heads, kv_heads, page, rope_d
     # the bytes lie where the header says, and nothing else was written
     tb = ref.tile_bytes(fmt, hd)
     pool = p.pool.cpu().numpy().reshape(p.n_pages, kv_heads, page // 16, tb)
-    seq = np.repeat(np.arange(4), rows)
+    seq = np.repeat(np.arange(len(rows)), rows)
     for i in rng.choice(n, 6, replace=False):
         for h in range(kv_heads):
             tile = pool[p.table[seq[i], pos[i] // page], h, pos[i] % page // 16]
@@ -162,6 +162,55 @@ def test_append_stores_what_the_rules_say(fmt, hd, heads, kv_heads, page, rope_d
     written = n * kv_heads * tb // 16
     changed = int((p.pool != before).sum())
     assert changed <= written and changed > written // 2
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("hd,heads,kv_heads,page,rope_dim,halves,bf16", [
+    (128, 8, 2, 16, 128, False, False), (128, 4, 4, 64, 64, True, True), (64, 3, 1, 32, 64, True, False),
+    (96, 6, 3, 48, 96, True, False), (96, 2, 1, 16, 34, False, True), (256, 2, 2, 128, 256, True, False),
+    (256, 4, 1, 16, 0, False, False), (64, 2, 2, 16, 8, True, True)])
+def test_append_stores_what_the_rules_say(fmt, hd, heads, kv_heads, page, rope_dim, halves, bf16):
+    check_append(fmt, hd, heads, kv_heads, page, rope_dim, halves, bf16, [5, 0, 1, 40], [21, 7, 1, 140])
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("hd,heads,kv_heads,page,rope_dim,halves,bf16", [
+    (128, 17, 9, 32, 128, False, True), (128, 3, 1, 16, 64, True, False), (64, 5, 1, 64, 64, True, True), (64, 4, 3, 16, 6, False, False),
+    (96, 3, 3, 48, 96, True, True), (96, 2, 1, 16, 34, False, False), (256, 3, 1, 128, 256, False, True),
+    (256, 2, 5, 16, 200, True, False), (256, 1, 1, 16, 0, True, False), (128, 33, 1, 16, 8, True, True)])
+@pytest.mark.parametrize("rows,lens", [([801], [801]), ([5, 0, 400, 1, 430], [21, 0, 713, 1, 439])])
+def test_append_of_many_rows(fmt, hd, heads, kv_heads, page, rope_dim, halves, bf16, rows, lens):
+    """Enough rows for whole tiles at a time, whose sequences begin and end inside tiles."""
+    check_append(fmt, hd, heads, kv_heads, page, rope_dim, halves, bf16, rows, lens)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_rows_and_tiles_leave_the_same_bytes(fmt):
+    """A prompt at once, and the same in pieces that are stored row by row."""
+    import torch
+    rng = np.random.default_rng(14)
+    hd, kv, n, far = 128, 3, 900, 70
+    x = torch_of(rng.standard_normal((n, 2 * kv * hd)).astype(np.float32))
+    freq, gain = capi.rope_frequencies(hd, 10000.0)
+    f = torch_of(freq)
+    rope, stride = capi.Rope(hd, 0, f.data_ptr(), gain), 2 * kv * hd
+    pools, backs = [], []
+    for steps in ([n], [150] * 6):
+        p = Paged(fmt, kv, hd, 64, [far + n], spare=0)
+        done = 0
+        for r in steps:
+            at = x.data_ptr() + done * stride * 4
+            p.cache.append(p.batch([r], [far + done + r]), rope, 0, 0, 0, 0, at, stride, at + kv * hd * 4, stride, 0, 0, 0)
+            done += r
+        pools.append(p.pool)
+        back = torch.empty(2, n, kv * hd, device="cuda")
+        done = 0
+        for r in steps:
+            p.cache.read(p.batch([r], [far + done + r]), back[0, done].data_ptr(), kv * hd, back[1, done].data_ptr(), kv * hd, 0)
+            done += r
+        backs.append(back)
+        assert capi.kernel_status(0) == 0
+    assert torch.equal(pools[0], pools[1]) and torch.equal(*backs)
 
 
 @pytest.mark.parametrize("fmt", FMTS)
@@ -228,6 +277,26 @@ def test_values_that_no_block_holds(fmt):
     np.testing.assert_array_equal(np_of(out)[0], want)
     np.testing.assert_array_equal(np_of(out)[1], want)
     assert np.isnan(want[0, :32]).all() and np.isfinite(want[0, 32:]).all() and np.isfinite(want[2:]).all()
+
+
+@pytest.mark.parametrize("fmt", [ref.Q4_0, ref.Q8_0])
+def test_values_that_no_block_holds_among_many_rows(fmt):
+    import torch
+    hd, n = 128, 807
+    v = np.random.default_rng(5).standard_normal((n, 1, hd)).astype(np.float32)
+    v[0, 0, 3], v[17, 0, 40], v[31, 0, 127] = np.inf, np.nan, -np.inf
+    v[33, 0, :32], v[400, 0, :32], v[806, 0, 5] = 3e38, 1e-9, -1e30
+    p = Paged(fmt, 1, hd, 32, [n])
+    x = torch_of(v.reshape(n, hd))
+    b = p.batch([n], [n])
+    p.cache.append(b, None, 0, 0, 0, 0, x.data_ptr(), hd, x.data_ptr(), hd, 0, 0, 0)
+    out = torch.empty(2, n, hd, device="cuda")
+    p.cache.read(b, out[0].data_ptr(), hd, out[1].data_ptr(), hd, 0)
+    assert capi.kernel_status(0) == 0
+    want = ref.stored(v, fmt).astype(np.float32)[:, 0]
+    np.testing.assert_array_equal(np_of(out)[0], want)
+    np.testing.assert_array_equal(np_of(out)[1], want)
+    assert int(np.isnan(want).sum()) == 3 * 32
 
 
 # ---- attention -----------------------------------------------------------------------------------------------------------
@@ -495,7 +564,7 @@ def check_prompt(p, rows, lens, heads, rng, bf16=False, window=0, q_scale=2.0, p
     q = (rng.standard_normal((sum(rows), heads, p.hd)) * q_scale).astype(np.float32)
     if bf16:
         q = ref.bf16_round(q)
-    got = p.attend(q, rows, lens, heads, bf16, True, window)
+    got = p.attend(q, rows, lens, heads, bf16, True, window, prompt=True)
     at, off, size = 0, 0.0, 0.0
     for s, (n, r) in enumerate(zip(lens, rows)):
         if r == 0:
@@ -539,7 +608,7 @@ def test_prompts_whose_scores_grow_along_the_keys():
     kd, vd = torch_of(k), torch_of(v)
     p.cache.append(p.batch([n], [n]), None, 0, 0, 0, 0, kd.data_ptr(), hd, vd.data_ptr(), hd, 0, 0, 0)
     q = rng.standard_normal((128, 2, hd)).astype(np.float32) * 4
-    got = p.attend(q, [128], [n], 2, out_bf16=True)
+    got = p.attend(q, [128], [n], 2, out_bf16=True, prompt=True)
     kk, vv = ref.stored(k, ref.F16), ref.stored(v, ref.F16)
     want = ref.attention(q, kk, vv, n, hd ** -0.5)
     assert np.linalg.norm(got - want) <= np.linalg.norm(want) * ref.norm_bound(hd, 4.0, 4.0, True)
@@ -556,7 +625,7 @@ def test_prompts_what_a_row_does_not_see_does_not_reach_it(fmt):
     kd, vd = torch_of(k), torch_of(v)
     p.cache.append(p.batch([n], [n]), None, 0, 0, 0, 0, kd.data_ptr(), hd, vd.data_ptr(), hd, 0, 0, 0)
     q = rng.standard_normal((rows, heads, hd)).astype(np.float32)
-    got = p.attend(q, [rows], [n], heads, out_bf16=True, window=100)
+    got = p.attend(q, [rows], [n], heads, out_bf16=True, prompt=True, window=100)
     pos = np.arange(n - rows, n)
     sees = ((pos >= 250) & (pos < 350)) | (pos >= 330)
     assert np.isfinite(got[~sees]).all() and not np.isfinite(got[sees][:, :, 70]).any()
@@ -572,7 +641,7 @@ def test_prompts_rows_that_see_nothing_and_padding(fmt):
     p = Paged(fmt, 1, 64, 16, [30, 0])
     ks, vs = p.fill(rng)
     q = rng.standard_normal((250, 2, 64)).astype(np.float32)
-    got = p.attend(q, [130, 70], [30, 0], 2, out_bf16=True, total=250)
+    got = p.attend(q, [130, 70], [30, 0], 2, out_bf16=True, prompt=True, total=250)
     assert (got[:100] == 0).all() and (got[130:200] == 0).all() and (got[200:] == 7).all()
     want = ref.attention(q[100:130], ks[0], vs[0], 30, 0.125)
     assert np.linalg.norm(got[100:130] - want) <= np.linalg.norm(want) * ref.norm_bound(64, 1.0, 1.0, True)
@@ -584,9 +653,9 @@ def test_prompts_repeat_bit_for_bit_and_leave_the_workspace_clean():
     p = Paged(ref.Q4_0, 4, 64, 16, [600, 200])
     p.fill(rng)
     q = rng.standard_normal((700, 8, 64)).astype(np.float32)
-    first = p.attend(q, [500, 200], [600, 200], 8, out_bf16=True)
+    first = p.attend(q, [500, 200], [600, 200], 8, out_bf16=True, prompt=True)
     for _ in range(3):
-        np.testing.assert_array_equal(p.attend(q, [500, 200], [600, 200], 8, out_bf16=True), first)
+        np.testing.assert_array_equal(p.attend(q, [500, 200], [600, 200], 8, out_bf16=True, prompt=True), first)
     assert int(p.workspace[:16384].to(torch.int32).sum()) == 0
 
 
@@ -597,19 +666,20 @@ def test_prompts_bad_pages_and_rows():
     ks, vs = p.fill(rng)
     good = p.table_dev.clone()
     q = rng.standard_normal((200, 2, 64)).astype(np.float32)
-    qd, out = torch_of(q.reshape(200, -1)), torch.zeros(200, 128, device="cuda", dtype=torch.bfloat16)
+    qd, out = torch.zeros(2048, 128, device="cuda"), torch.zeros(2048, 128, device="cuda", dtype=torch.bfloat16)
+    qd[:200] = torch_of(q.reshape(200, -1))
 
     def attend(b):
         p.cache.attend(b, 2, qd.data_ptr(), 0, 128, out.data_ptr(), 1, 128, 0.125, 0, p.workspace.data_ptr())
 
     for page in (-1, p.n_pages):
         p.table_dev[0, 5] = page
-        assert "21" in status_of(lambda: attend(p.batch([100, 100], [200, 200])))
+        assert "21" in status_of(lambda: attend(p.batch([100, 100], [200, 200], total=2048)))
         want = ref.attention(q[100:], ks[1], vs[1], 200, 0.125)
-        assert np.linalg.norm(np_of(out)[100:].reshape(100, 2, 64) - want) <= np.linalg.norm(want) * ref.norm_bound(64, 1.0, 1.0, True)
+        assert np.linalg.norm(np_of(out)[100:200].reshape(100, 2, 64) - want) <= np.linalg.norm(want) * ref.norm_bound(64, 1.0, 1.0, True)
     p.table_dev.copy_(good)
-    assert "22" in status_of(lambda: attend(p.batch([100, 100], [p.width * 16 + 1, 200])))
-    assert "22" in status_of(lambda: attend(p.batch([100, 150], [200, 200], total=200)))
+    assert "22" in status_of(lambda: attend(p.batch([100, 100], [p.width * 16 + 1, 200], total=2048)))
+    assert "22" in status_of(lambda: attend(p.batch([100, 1949], [200, 2000], total=2048)))
     assert int(p.workspace[:16384].to(torch.int32).sum()) == 0
 
 
@@ -663,6 +733,46 @@ def test_bad_pages_and_rows_are_skipped_and_reported(fmt):
     for s in range(2):
         want = ref.attention(q[s:s + 1], ks[s], vs[s], 40, 0.125)
         assert np.abs(got[s] - want[0]).max() <= ref.attention_bound(q, ks[s], vs[s], 0.125, False)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_bad_pages_and_rows_among_many_rows(fmt):
+    """Whole tiles at a time: what is bad is left out and reported, the rest is stored."""
+    import torch
+    rng = np.random.default_rng(26)
+    rows, hd = [420, 0, 420], 64
+    p = Paged(fmt, 1, hd, 32, [440, 3, 420])
+    x = torch_of(rng.standard_normal((840, hd)).astype(np.float32))
+    back = torch.full((2, 840, hd), 5.0, device="cuda")
+
+    def append(b):
+        p.cache.append(b, None, 0, 0, 0, 0, x.data_ptr(), hd, x.data_ptr(), hd, 0, 0, 0)
+
+    def read(b):
+        p.cache.read(b, back[0].data_ptr(), hd, back[1].data_ptr(), hd, 0)
+
+    b = p.batch(rows, p.lens)
+    good = int(p.table_dev[0, 4])
+    for page in (-1, p.n_pages, 2 ** 31 - 1):
+        p.table_dev[0, 4] = page  # positions 128 to 159, rows 108 to 139
+        assert "21" in status_of(lambda: append(b))
+        assert "21" in status_of(lambda: read(b))
+    want = ref.stored(x.cpu().numpy().reshape(840, 1, hd), fmt).astype(np.float32)[:, 0]
+    want[108:140] = 5.0
+    np.testing.assert_array_equal(np_of(back)[0], want)
+    np.testing.assert_array_equal(np_of(back)[1], want)
+    p.table_dev[0, 4] = good
+    pool = p.pool.clone()
+    for lens, begin in (([419, 3, 419], None), ([-1, 3, 2 ** 30], None), ([440, 3, 420], [0, -3, 2 ** 30, 840]),
+                        ([440, 3, 420], [9, 4, 2, -1])):
+        b = p.batch(rows, lens)
+        if begin is not None:
+            t = torch.tensor(begin, dtype=torch.int32, device="cuda")
+            p.hold.append(t)
+            b.row_begin_dev = t.data_ptr()
+        assert "22" in status_of(lambda: append(b))
+        assert "22" in status_of(lambda: read(b))
+    assert torch.equal(p.pool, pool)
 
 
 def test_empty_calls_do_nothing():

@@ -187,5 +187,9 @@ def test_paged_fp16_equals_the_contiguous_cache(stream):
         got.append((model.last_logits(), model.batch_decode(12)))
         model.close()
     (l0, t0), (l1, t1) = got
-    assert apart(l1, l0) <= 1e-3
+    # The contiguous cache's prompts round probabilities to fp16, a call of so few rows over pages does not: a context value is off
+    # by up to 2^-11 of sum p |v|, twice that of itself where v's signs differ.  Both are then rounded to bf16, steps of up to 2^-7:
+    # a value that is off by 2^-10 lands a step away once in 8 times, a 2-norm of sqrt(2^-10 * 2^-7) = 2^-8.5 of the context, and
+    # two layers' add up to 2^-8.  (A bound of 1e-3 held only as long as both sides rounded the probabilities.)
+    assert apart(l1, l0) <= 2.0 ** -8
     assert (t0 == t1).mean() > 0.9
