@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
                 const KvSeq q = kv_seq(a.pool, a.seqs, s, bad);
                 n = ((long long)q.n * a.group + COLS - 1) / COLS * a.pool.kv_heads;
             }
-            if (bad && blockIdx.x == 0 && first) {
+            if (bad) {  // the fetch that finds no item has seen every sequence
                 atomicExch(a.seqs.status, KV_BAD_ROWS);
             }
             long long upto = n;
@@ -342,52 +342,67 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
         }
         // ---- queries ----
         else {
-            constexpr int EACH = HD / 32, AT_ONCE = 8;  // consecutive dimensions of a lane, columns in flight
-            constexpr int MINE = COLS / (SOFT_WARPS + KV_WARPS);
-            for (int c8 = 0; c8 < MINE; c8 += AT_ONCE) {
-                float v[AT_ONCE][EACH];
+            // Eight lanes to a column, which take four dimensions of every 32 each: four columns share what a column costs beside its
+            // values (a warp to a column: 8 us for an item's queries).  Loads go without branches, to column 0 in place of one that is
+            // not there.
+            constexpr int AT_ONCE = 2, MINE = COLS / (SOFT_WARPS + KV_WARPS);
+            const int j = lane & 7;
+            for (int c8 = 0; c8 < MINE; c8 += 4 * AT_ONCE) {
+                float v[AT_ONCE][NB][4];
+                const auto bring = [&](auto f32) {
 #pragma unroll
-                for (int k = 0; k < AT_ONCE; ++k) {
-                    const int c = warp * MINE + c8 + k;
-                    const bool on = c < it.cols;
-                    const int64_t row = it.q.row0 + (on ? (it.col0 + c) / a.group : 0);
-                    const int qh = it.head * a.group + (on ? (it.col0 + c) % a.group : 0);
-                    const int64_t src = row * a.q_stride + (int64_t)qh * HD + lane * EACH;
+                    for (int k = 0; k < AT_ONCE; ++k) {
+                        const int c = warp * MINE + c8 + 4 * k + (lane >> 3), col = it.col0 + (c < it.cols ? c : 0), row = col / a.group;
+                        const int64_t src = (it.q.row0 + row) * a.q_stride + (int64_t)(it.head * a.group + col - row * a.group) * HD + 4 * j;
 #pragma unroll
-                    for (int i = 0; i < EACH; i += 2) {
-                        float2 x = make_float2(0.0f, 0.0f);
-                        if (on) {
-                            if (a.q_type == QMM_OUT_F32) {
-                                x = *reinterpret_cast<const float2*>(static_cast<const float*>(a.q) + src + i);
+                        for (int n = 0; n < NB; ++n) {
+                            if (decltype(f32)::value) {
+                                const float4 x = *reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + src + 32 * n);
+                                v[k][n][0] = x.x, v[k][n][1] = x.y, v[k][n][2] = x.z, v[k][n][3] = x.w;
                             } else {
-                                x = __bfloat1622float2(
-                                    *reinterpret_cast<const __nv_bfloat162*>(static_cast<const __nv_bfloat16*>(a.q) + src + i));
+                                const uint2 x = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(a.q) + src + 32 * n);
+                                v[k][n][0] = __uint_as_float(x.x << 16), v[k][n][1] = __uint_as_float(x.x & 0xFFFF0000u);
+                                v[k][n][2] = __uint_as_float(x.y << 16), v[k][n][3] = __uint_as_float(x.y & 0xFFFF0000u);
                             }
                         }
-                        v[k][i] = x.x, v[k][i + 1] = x.y;
                     }
+                };
+                if (a.q_type == QMM_OUT_F32) {
+                    bring(std::true_type{});
+                } else {
+                    bring(std::false_type{});
                 }
 #pragma unroll
                 for (int k = 0; k < AT_ONCE; ++k) {
-                    const int c = warp * MINE + c8 + k;
+                    const int c = warp * MINE + c8 + 4 * k + (lane >> 3);
                     uint32_t bits = 0;
 #pragma unroll
-                    for (int i = 0; i < EACH; ++i) {
-                        bits = max(bits, __float_as_uint(v[k][i]) & 0x7FFFFFFFu);
+                    for (int n = 0; n < NB; ++n) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            v[k][n][i] = c < it.cols ? v[k][n][i] : 0.0f;
+                            bits = max(bits, __float_as_uint(v[k][n][i]) & 0x7FFFFFFFu);
+                        }
                     }
-                    bits = __reduce_max_sync(0xFFFFFFFFu, bits);
+#pragma unroll
+                    for (int o = 1; o < 8; o <<= 1) {
+                        bits = max(bits, __shfl_xor_sync(0xFFFFFFFFu, bits, o));
+                    }
                     const int exponent = (int)(bits >> 23) - 127;
                     const int e = bits == 0 || exponent == 128 ? 0 : max(-112, min(120, 12 - exponent));
                     const float up = __uint_as_float((uint32_t)(e + 127) << 23 | (a.scale < 0.0f ? 0x80000000u : 0u));
                     uint8_t* row = q_smem + (c / M_TILE) * Shape::Q_BYTES + (c % M_TILE) * 128;
 #pragma unroll
-                    for (int i = 0; i < EACH; i += 2) {
-                        // dimension 32 n + 8 t + 2 r + e lies at 32 n + 8 r + 2 t + e, as in the keys
-                        const int dim = lane * EACH + i, chunk = (dim % 64) / 32 * 4 + dim / 2 % 4;
-                        *reinterpret_cast<__half2*>(row + dim / 64 * (M_TILE * 128) + ((chunk ^ (c & 7)) << 4) + dim / 8 % 4 * 4) =
-                            __floats2half2_rn(v[k][i] * up, v[k][i + 1] * up);
+                    for (int n = 0; n < NB; ++n) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            // dimension 32 n + 8 t + 2 r + e lies at 32 n + 8 r + 2 t + e, as in the keys: t is j / 2, r is 2 (j % 2) + h
+                            const int chunk = n % 2 * 4 + 2 * (j & 1) + h;
+                            *reinterpret_cast<__half2*>(row + n / 2 * (M_TILE * 128) + ((chunk ^ (c & 7)) << 4) + (j >> 1) * 4) =
+                                __floats2half2_rn(v[k][n][2 * h] * up, v[k][n][2 * h + 1] * up);
+                        }
                     }
-                    if (lane == 0) {
+                    if (j == 0) {
                         ctl.q_scale[c] = fabsf(a.scale) * 1.44269504088896340736f * __uint_as_float((uint32_t)(127 - e) << 23);
                     }
                 }
@@ -801,7 +816,12 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
             }
             const int64_t row = it.q.row0 + (it.col0 + c) / a.group;
             const int qh = it.head * a.group + (it.col0 + c) % a.group;
-            __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + row * a.out_stride + (int64_t)qh * HD;
+            const unsigned long long out = c < it.cols && ok
+                                               ? reinterpret_cast<unsigned long long>(static_cast<__nv_bfloat16*>(a.out) + row * a.out_stride + (int64_t)qh * HD)
+                                               : 0ull;
+            // The queries' place, which the products have left (o_full), takes a column's row, so that a warp writes whole rows: 16
+            // bytes of 32 rows at a time took 3 us an item.
+            uint8_t* place = q_smem + i * Shape::Q_BYTES + (c % M_TILE) * 128;
             const bool none = my_blocks == 0 || (m == -INFINITY && l == 0.0f);
             const float inv = none ? 0.0f : poisoned ? __uint_as_float(0x7FC00000u) : 1.0f / l;
 #pragma unroll
@@ -813,7 +833,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
                     tmem_wait_ld(o[0]);
                     tmem_wait_ld(o[1]);
                 }
-                if (c < it.cols && ok) {
+                if (ok) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {  // dimensions 32 n + 8 k ..: 4 g + j is column 8 j + g
                         uint32_t x[4];
@@ -824,8 +844,20 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
                             const __nv_bfloat162 pair = __floats2bfloat162_rn(x0, x1);
                             x[h] = *reinterpret_cast<const uint32_t*>(&pair);
                         }
-                        *reinterpret_cast<uint4*>(out + 32 * n + 8 * k) = make_uint4(x[0], x[1], x[2], x[3]);
+                        *reinterpret_cast<uint4*>(place + n / 2 * (M_TILE * 128) + (((n % 2 * 4 + k) ^ (c & 7)) << 4)) =
+                            make_uint4(x[0], x[1], x[2], x[3]);
                     }
+                }
+            }
+            __syncwarp();
+            constexpr int LANES = HD / 8;  // of a row, 16 bytes each
+#pragma unroll
+            for (int r = 0; r < LANES; ++r) {
+                const int from = r * (32 / LANES) + lane / LANES, chunk = lane % LANES, cc = (warp & 3) * 32 + from;
+                const unsigned long long to = __shfl_sync(0xFFFFFFFFu, out, from);
+                if (to != 0) {
+                    reinterpret_cast<uint4*>(to)[chunk] = *reinterpret_cast<const uint4*>(
+                        q_smem + i * Shape::Q_BYTES + chunk / 8 * (M_TILE * 128) + cc * 128 + ((chunk % 8 ^ (cc & 7)) << 4));
                 }
             }
             fence_before();
