@@ -258,7 +258,8 @@ __device__ __forceinline__ RowPlace find_row(const KvPool& c, const KvSeqs& b, i
     return p;
 }
 
-// One row per blockIdx.y, its work cut over blockIdx.x.  Simple form: every thread takes four dimensions of a head.
+// One row per blockIdx.y, its work cut over blockIdx.x: every thread takes four dimensions of a head.  For few rows, where a call's
+// time is its latency: one token of 8 kv heads of 128 and 32 query heads 3.0 us in Q4_0, 16 tokens 3.3 us (its bytes would take 0.1 us).
 template <int FMT>
 __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendArgs a)
 {
@@ -522,7 +523,12 @@ __device__ __forceinline__ void turn_halves(const KvAppendArgs& a, const double2
     }
 }
 
-// blockIdx.x: groups of kv heads, then groups of query heads; blockIdx.y: tiles.
+// Many rows.  blockIdx.x: groups of kv heads, then groups of query heads; blockIdx.y: tiles.  A warp takes a row at a time.  A whole
+// tile is put together in shared memory: stored from the registers, its two- and four-byte pieces made a sector of DRAM traffic
+// each.  Bound: 1999 rows of 32 heads of 128 with as many kv heads, fp32 to Q4_0, move 170 MB in 64 us (41 % of the copy rate) with half of the issue
+// slots taken: rotation and its conversions in fp64, and the blocks' quants.  Sixteen prompts of 33 to 901 rows, 64 query and 8 kv
+// heads of 128, half of each rotated, bf16 to fp16: 124 us (42 %).  Registers for three CTAs of an SM: two left loads exposed (218 us), four
+// spill (144 us).  Sixteen warps a CTA: 64 and 147 us.
 template <int FMT, int HD, bool HALVES>
 __global__ void __launch_bounds__(TILE_WARPS * 32, 24 / TILE_WARPS) kv_append_tile_kernel(const KvAppendArgs a)
 {

@@ -4,10 +4,11 @@
 // A tile holds 16 tokens of one kv head: key quants, key scales, value quants, value scales.  The quant planes are in the order
 // in which the attention kernels' MMA operands want them, so that a lane reads its share of a tile as whole vectors without
 // shuffles, and a tile is one run of bytes that one bulk copy brings in:
-//   keys    B operand of q . K^T (mma m16n8k16, n = token): lane 4g + t holds, for token 8j + g, the eight dimensions
-//           32b + 8t + {0..7} of every block b.  A block is two k16 steps, so its scale meets the sum of exactly two MMAs.
-//   values  B operand of P . V (n = dimension, k = token): lane 4g + t holds, for tokens 8j + 2t and 8j + 2t + 1, the four
+//   keys    A operand of K . q^T (mma m16n8k16, row = token): lane 4g + t holds, for tokens g and g + 8 (half j = 0, 1), the eight
+//           dimensions 32b + 8t + {0..7} of every block b.  A block is two k16 steps, so its scale meets the sum of exactly those.
+//   values  A operand of V^T . P^T (row = dimension, k = token): lane 4g + t holds, for tokens 8j + 2t and 8j + 2t + 1, the four
 //           dimensions 32b + 4g + {0..3} of every block, the two tokens' values of a dimension in one 32-bit operand register.
+// The prompt kernel stores the same registers as 8 x 8 matrices.
 #pragma once
 
 #include <cuda_bf16.h>
