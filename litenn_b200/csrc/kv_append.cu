@@ -384,48 +384,59 @@ struct TilePlace {
     int seq, pos0, begin, end;  // seq < 0: there is no such tile
     int64_t row;
 };
-// The `want`-th tile over all sequences.  Whole CTA; reports what is bad.
+// The `want`-th tile over all sequences.  Whole CTA; the first reports what is bad.  A lane counts the tiles of batch / 32 sequences in
+// a row, and the one that has the tile counts again.
 __device__ __forceinline__ TilePlace find_tile(const KvPool& c, const KvSeqs& b, int64_t want, TilePlace* shared)
 {
     if (threadIdx.x < 32) {
-        const int lane = threadIdx.x;
-        TilePlace p = {-1, 0, 0, 0, 0};
-        int64_t before = 0;
-        for (int base = 0; base < b.batch && p.seq < 0 && before <= want; base += 32) {
-            const int s = base + lane;
-            bool bad = false;
-            KvSeq q = {0, 0, 0};
-            if (s < b.batch) {
-                q = kv_seq(c, b, s, bad);
-                bad = bad || q.len < q.n;
-            }
-            if (bad) {
-                q.n = 0;
-                atomicExch(b.status, KV_BAD_ROWS);
-            }
-            const int first = q.len - q.n, t0 = q.n > 0 ? first / KV_TILE : 0;
-            int64_t upto = q.n > 0 ? (q.len - 1) / KV_TILE - t0 + 1 : 0;
-            const int64_t mine = upto;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int64_t u = __shfl_up_sync(0xFFFFFFFFu, upto, o);
-                upto += lane >= o ? u : 0;
-            }
-            const bool here = mine > 0 && before + upto - mine <= want && want < before + upto;
-            if (here) {
-                const int tile = t0 + (int)(want - (before + upto - mine));
-                p.seq = s;
-                p.pos0 = tile * KV_TILE;
-                p.begin = max(0, first - p.pos0);
-                p.end = min(KV_TILE, q.len - p.pos0);
-                p.row = q.row0 + (p.pos0 + p.begin - first);
-                *shared = p;
-            }
-            p.seq = __any_sync(0xFFFFFFFFu, here) ? 0 : -1;
-            before += __shfl_sync(0xFFFFFFFFu, upto, 31);
+        const int lane = threadIdx.x, each = (b.batch + 31) / 32, s0 = lane * each, s1 = min(b.batch, s0 + each);
+        const auto look = [&](int s, bool& bad) {
+            KvSeq q = kv_seq(c, b, s, bad);
+            bad = bad || q.len < q.n;
+            q.n = bad ? 0 : q.n;
+            return q;
+        };
+        const auto tiles = [](const KvSeq& q) { return q.n > 0 ? (q.len - 1) / KV_TILE - (q.len - q.n) / KV_TILE + 1 : 0; };
+        int64_t mine = 0;
+        bool any_bad = false;
+#pragma unroll 4
+        for (int s = s0; s < s1; ++s) {
+            bool bad;
+            mine += tiles(look(s, bad));
+            any_bad = any_bad || bad;
         }
-        if (p.seq < 0 && lane == 0) {
-            *shared = p;
+        if (any_bad && want == 0) {
+            atomicExch(b.status, KV_BAD_ROWS);
+        }
+        int64_t upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t u = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+            upto += lane >= o ? u : 0;
+        }
+        int64_t before = upto - mine;
+        const bool here = before <= want && want < upto;
+        if (here) {
+            for (int s = s0; s < s1; ++s) {
+                bool bad;
+                const KvSeq q = look(s, bad);
+                const int n = tiles(q);
+                if (want < before + n) {
+                    TilePlace p;
+                    const int first = q.len - q.n, tile = first / KV_TILE + (int)(want - before);
+                    p.seq = s;
+                    p.pos0 = tile * KV_TILE;
+                    p.begin = max(0, first - p.pos0);
+                    p.end = min(KV_TILE, q.len - p.pos0);
+                    p.row = q.row0 + (p.pos0 + p.begin - first);
+                    *shared = p;
+                    break;
+                }
+                before += n;
+            }
+        }
+        if (!__any_sync(0xFFFFFFFFu, here) && lane == 0) {
+            shared->seq = -1;
         }
     }
     __syncthreads();

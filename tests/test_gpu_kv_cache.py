@@ -184,6 +184,40 @@ def test_append_of_many_rows(fmt, hd, heads, kv_heads, page, rope_dim, halves, b
     check_append(fmt, hd, heads, kv_heads, page, rope_dim, halves, bf16, rows, lens)
 
 
+def test_append_of_many_sequences_of_many_rows():
+    """More sequences than lanes count at once, empty ones and an impossible one among them."""
+    import torch
+    rng = np.random.default_rng(15)
+    rows = [int(r) for r in rng.integers(0, 40, 150)]
+    lens = [r + int(e) for r, e in zip(rows, rng.integers(0, 30, 150))]
+    assert sum(rows) > 8 * 150
+    hd = 64
+    p = Paged(ref.Q8_0, 1, hd, 16, lens)
+    x = torch_of(rng.standard_normal((sum(rows), hd)).astype(np.float32))
+    back = torch.full((2, sum(rows), hd), 5.0, device="cuda")
+    bad = 77
+    assert rows[bad] > 0
+    wrong = list(lens)
+    wrong[bad] = rows[bad] - 1
+    for given, message in ((wrong, "22"), (lens, None)):
+        b = p.batch(rows, given)
+
+        def both():
+            p.cache.append(b, None, 0, 0, 0, 0, x.data_ptr(), hd, x.data_ptr(), hd, 0, 0, 0)
+            p.cache.read(b, back[0].data_ptr(), hd, back[1].data_ptr(), hd, 0)
+
+        want = ref.stored(x.cpu().numpy().reshape(-1, 1, hd), ref.Q8_0).astype(np.float32)[:, 0]
+        if message:
+            assert message in status_of(both)
+            at = sum(rows[:bad])
+            want[at:at + rows[bad]] = 5.0
+        else:
+            both()
+            assert capi.kernel_status(0) == 0
+        np.testing.assert_array_equal(np_of(back)[0], want)
+        np.testing.assert_array_equal(np_of(back)[1], want)
+
+
 @pytest.mark.parametrize("fmt", FMTS)
 def test_rows_and_tiles_leave_the_same_bytes(fmt):
     """A prompt at once, and the same in pieces that are stored row by row."""
