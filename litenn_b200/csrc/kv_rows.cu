@@ -21,8 +21,8 @@
 // What bounds it beside the bytes: instructions, about 415 a warp for a Q4_0 tile of 128 dimensions (issue 60 to 70 % of the
 // slots), and 12 to 15 us of a call that its length does not change (the lengths' scan 1.5, queries and pages 3, joining warps
 // and CTAs 3 to 5).  One token, us: 131072 tokens of 8 kv heads of 128 in Q4_0, 64 heads 61 (2.5 TB/s; its copies alone 45), 16 sequences of
-// 700 to 8191 tokens 45, 639 tokens of 32 kv heads 14; 16 sequences of 500 to 2000 tokens of 32 kv heads in fp16 64 (5.1 TB/s, 78 %
-// of the copy rate); 8 sequences of 100 to 4000 tokens in Q8_0, 3 to 5 rows each of 32 heads, 29.
+// 700 to 8191 tokens 44, 639 tokens of 32 kv heads 14; 16 sequences of 500 to 2000 tokens of 32 kv heads in fp16 63 (5.2 TB/s, 79 %
+// of the copy rate); 8 sequences of 100 to 4000 tokens in Q8_0, 3 to 5 rows each of 32 heads, 28.
 //
 // Work is cut evenly (kv_rows_plan.cuh) on the device, from the lengths, so that ragged batches and single long sequences both
 // fill the GPU and a captured launch follows the lengths.  Where a list entry spans CTAs, each leaves its part in the workspace
