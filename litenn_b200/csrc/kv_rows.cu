@@ -481,13 +481,13 @@ __global__ void __launch_bounds__(RowsShape<FMT, HD, NT>::WARPS * 32, RowsShape<
             qs[n] = *reinterpret_cast<const float2*>(qscale + 8 * n + 2 * t);
             m[n] = make_float2(-INFINITY, -INFINITY);
             l[n] = make_float2(0.0f, 0.0f);
-            // columns past `cols` see what comes, unstored
-            pos_of[n][0] = first_pos + (col0 + 8 * n + 2 * t) / a.group;
-            pos_of[n][1] = first_pos + (col0 + 8 * n + 2 * t + 1) / a.group;
-            op_pos[n] = first_pos + (col0 + 8 * n + g) / a.group;
+            // columns past `cols` see what comes, unstored; rows in front of the first token see nothing
+            pos_of[n][0] = max(-1, first_pos + (col0 + 8 * n + 2 * t) / a.group);
+            pos_of[n][1] = max(-1, first_pos + (col0 + 8 * n + 2 * t + 1) / a.group);
+            op_pos[n] = max(-1, first_pos + (col0 + 8 * n + g) / a.group);
         }
         const int key_scale_at = kv_scale_place(HD, g, 0);  // of token g; token g + 8 and block b are a constant away
-        const int reach = a.window > 0 ? a.window - 1 : 0x3FFFFFFF;  // a row at pos sees pos - reach .. pos
+        const int reach = a.window > 0 ? a.window - 1 : 0x7FFFFFFF;  // a row at pos sees pos - reach .. pos
         float o[NT][HD / 16][4] = {};
         float vs = 0.0f;      // power of two that brings value scales near one
         uint32_t limit = 0;   // fp16 bits: scales above it lower vs
