@@ -693,6 +693,68 @@ def test_prompts_repeat_bit_for_bit_and_leave_the_workspace_clean():
     assert int(p.workspace[:16384].to(torch.int32).sum()) == 0
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+def test_prompts_captured_once_follow_rows_and_lengths(fmt):
+    """Tiles appended and prompts attended in one graph, whose rows are cut differently at every replay."""
+    import torch
+    rng = np.random.default_rng(27)
+    hd, heads, kv, total = 64, 4, 2, 1024
+    p = Paged(fmt, kv, hd, 32, [total] * 3)
+    width = heads + 2 * kv
+    qkv = rng.standard_normal((total, width, hd)).astype(np.float32)
+    x, freq = torch_of(qkv.reshape(total, -1)), capi.rope_frequencies(hd, 10000.0)[0]
+    f = torch_of(freq)
+    rope, stride = capi.Rope(hd, 1, f.data_ptr(), 1.0), width * hd
+    q = torch.zeros(total, heads * hd, device="cuda")
+    out = torch.zeros(total, heads * hd, device="cuda", dtype=torch.bfloat16)
+    begin, length = (torch.zeros(n, device="cuda", dtype=torch.int32) for n in (4, 3))
+    b = capi.KVBatch(3, p.width, p.table_dev.data_ptr(), length.data_ptr(), begin.data_ptr(), total)
+    stream, at = torch.cuda.Stream(), x.data_ptr()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(stream):
+        with torch.cuda.graph(graph, stream=stream):
+            p.cache.append(b, rope, heads, 0, at, stride, at + heads * hd * 4, stride, at + (heads + kv) * hd * 4, stride,
+                           q.data_ptr(), 0, heads * hd, stream.cuda_stream)
+            p.cache.attend(b, heads, q.data_ptr(), 0, heads * hd, out.data_ptr(), 1, heads * hd, 0.125, 0,
+                           p.workspace.data_ptr(), stream.cuda_stream)
+    for rows in ([300, 0, 200], [1, 700, 300], [0, 0, 0], [513, 31, 33]):
+        cut = np.concatenate([[0], np.cumsum(rows)])
+        begin.copy_(torch_of(cut.astype(np.int32)))
+        length.copy_(torch_of(np.asarray(rows, dtype=np.int32)))
+        out.fill_(7.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = np_of(out).reshape(total, heads, hd)
+        assert (got[cut[-1]:] == 7.0).all()
+        for s, n in enumerate(rows):
+            if n:
+                part = qkv[cut[s]:cut[s + 1]]
+                turned = ref.rotate(part[:, :heads + kv], np.arange(n), freq, 1.0, hd, True)
+                keys, vals = ref.stored(turned[:, heads:], fmt), ref.stored(part[:, heads + kv:], fmt)
+                want = ref.attention(turned[:, :heads], keys, vals, n, 0.125)
+                assert np.abs(got[cut[s]:cut[s + 1]] - want).max() <= ref.attention_bound(turned[:, :heads], keys, vals, 0.125,
+                                                                                          True, True)
+    assert capi.kernel_status(0) == 0
+    del graph
+
+
+def test_prompts_queries_that_are_not_finite_stay_their_own_rows():
+    rng = np.random.default_rng(28)
+    n, rows, heads, hd = 300, 150, 2, 128
+    p = Paged(ref.Q4_0, 1, hd, 16, [n])
+    ks, vs = p.fill(rng)
+    q = rng.standard_normal((rows, heads, hd)).astype(np.float32)
+    q[3, 1, 5], q[140, 0, 127] = np.nan, np.inf
+    got = p.attend(q, [rows], [n], heads, out_bf16=True, prompt=True)
+    odd = np.zeros((rows, heads), dtype=bool)
+    odd[3, 1] = odd[140, 0] = True
+    assert np.isnan(got[odd]).all() and np.isfinite(got[~odd]).all()
+    want = ref.attention(np.nan_to_num(q, posinf=0.0), ks[0], vs[0], n, hd ** -0.5)
+    assert np.linalg.norm((got - want)[~odd]) <= np.linalg.norm(want) * ref.norm_bound(hd, 1.0, 1.0, True)
+
+
 def test_prompts_bad_pages_and_rows():
     rng = np.random.default_rng(25)
     import torch
