@@ -18,8 +18,8 @@
 // registers of sums instead of 64 at 128 dimensions, so four CTAs share an SM instead of three.  What it costs are four 8 x 8
 // transposes per tile that turn the scores' layout (row = token) into the probabilities' operand layout (row = column).
 //
-// What bounds it beside the bytes: instructions, about 415 a warp for a Q4_0 tile of 128 dimensions (issue 60 to 70 % of the
-// slots), and 12 to 15 us of a call that its length does not change (the lengths' scan 1.5, queries and pages 3, joining warps
+// What bounds it beside the bytes: instructions, about 415 a warp for a Q4_0 tile of 128 dimensions (57 % of the issue
+// slots, 3.6 warps a scheduler), and 12 to 15 us of a call that its length does not change (the lengths' scan 1.5, queries and pages 3, joining warps
 // and CTAs 3 to 5).  One token, us: 131072 tokens of 8 kv heads of 128 in Q4_0, 64 heads 61 (2.5 TB/s; its copies alone 45), 16 sequences of
 // 700 to 8191 tokens 44, 639 tokens of 32 kv heads 14; 16 sequences of 500 to 2000 tokens of 32 kv heads in fp16 63 (5.2 TB/s, 79 %
 // of the copy rate); 8 sequences of 100 to 4000 tokens in Q8_0, 3 to 5 rows each of 32 heads, 28.
