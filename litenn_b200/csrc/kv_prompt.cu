@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
                 n.first_pos = n.q.len - n.q.n;
                 const int pos_lo = n.first_pos + n.col0 / a.group;
                 n.pos_hi = n.first_pos + (n.col0 + n.cols - 1) / a.group;
-                n.seen_lo = a.window > 0 ? max(0, pos_lo - a.window + 1) : 0;
+                n.seen_lo = kv_first_seen(pos_lo, a.window);
                 n.k0 = n.seen_lo / KV_TILE * KV_TILE;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
@@ -686,7 +686,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
             const uint32_t s_at = tmem + lanes + i * BLOCK, o_at = tmem + lanes + 2 * BLOCK + i * M_TILE;
             const float qs = ctl.q_scale[c];
             const int pos = it.first_pos + (it.col0 + c) / a.group;
-            const int low = a.window > 0 ? pos - a.window + 1 : 0;
+            const int low = kv_first_seen(pos, a.window);
             float m = -INFINITY, l = 0.0f;
             bool ok = true, poisoned = false;
             const int my_blocks = it.blocks[i];

@@ -20,6 +20,12 @@ __host__ __device__ __forceinline__ int kv_min(int a, int b)
 {
     return a < b ? a : b;
 }
+// First position that a row at `pos` sees (window 0: no limit).  No difference is taken where it could leave 32 bits: rows in front of
+// a sequence's first token have negative positions, and a window may be 2^31 - 1.
+__host__ __device__ __forceinline__ int kv_first_seen(int pos, int window)
+{
+    return window > 0 && pos >= window ? pos - window + 1 : 0;
+}
 // Division of numbers below 2^63, in 32 bits where they fit (a 64-bit division is a hundred dependent instructions, and a short
 // call waits for half a dozen of them).
 __host__ __device__ __forceinline__ long long kv_div(long long x, long long y)
@@ -45,8 +51,7 @@ __host__ __device__ __forceinline__ SeqWork seq_work(const KvPool& c, const KvSe
     // tiles from the first that the first row's window reaches to the last token's; a sequence without any still has its
     // rows' zeros to write
     const int first = x.q.len - x.q.n;
-    const int low = window > 0 ? kv_max(0, first - window + 1) : 0;
-    x.tile0 = low / KV_TILE;
+    x.tile0 = kv_first_seen(first, window) / KV_TILE;
     x.tiles = kv_max(1, (x.q.len + KV_TILE - 1) / KV_TILE - x.tile0);
     x.passes = (int)(((long long)x.q.n * group + cols - 1) / cols);
     x.units = (long long)c.kv_heads * x.passes * (x.tiles + KV_ENTRY_UNITS);
@@ -70,8 +75,8 @@ __host__ __device__ __forceinline__ PassView pass_view(const SeqWork& x, int gro
     const int first = x.q.len - x.q.n;
     v.pos_lo = first + v.col0 / group;
     v.pos_hi = first + (v.col0 + v.cols - 1) / group;
-    v.seen_lo = window > 0 ? kv_max(0, v.pos_lo - window + 1) : 0;
-    v.all_lo = window > 0 ? kv_max(0, v.pos_hi - window + 1) : 0;
+    v.seen_lo = kv_first_seen(v.pos_lo, window);
+    v.all_lo = kv_first_seen(v.pos_hi, window);
     v.tile_begin = kv_max(tile_begin, v.seen_lo / KV_TILE);
     v.tile_end = kv_min(tile_end, v.pos_hi < 0 ? 0 : v.pos_hi / KV_TILE + 1);
     return v;

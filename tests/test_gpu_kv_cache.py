@@ -681,6 +681,21 @@ def test_prompts_rows_that_see_nothing_and_padding(fmt):
     assert np.linalg.norm(got[100:130] - want) <= np.linalg.norm(want) * ref.norm_bound(64, 1.0, 1.0, True)
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 4, 2 ** 30])
+@pytest.mark.parametrize("prompt", [False, True])
+def test_a_window_wider_than_any_sequence_is_none(fmt, window, prompt):
+    """With rows in front of the first token, in either kernel: the bits of a call without a window."""
+    rng = np.random.default_rng(31)
+    p = Paged(fmt, 1, 64, 16, [30, 3])
+    p.fill(rng)
+    q = rng.standard_normal((160, 4, 64)).astype(np.float32)
+    got = [p.attend(q, [150, 10], [30, 3], 4, out_bf16=prompt, prompt=prompt, window=w) for w in (0, window)]
+    sees = np.r_[120:150, 157:160]
+    assert got[0][sees].any(-1).all() and not np.delete(got[0], sees, 0).any()
+    np.testing.assert_array_equal(got[1], got[0])
+
+
 def test_prompts_repeat_bit_for_bit_and_leave_the_workspace_clean():
     rng = np.random.default_rng(24)
     import torch

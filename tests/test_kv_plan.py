@@ -61,6 +61,17 @@ def test_every_pair_is_visited_once(lib, rows, lens, group, kv_heads, window, gr
         at += r
 
 
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 4, 2 ** 30])
+@pytest.mark.parametrize("rows,lens", [([8], [3]), ([40], [20]), ([10, 1, 5], [5, 90, 0]), ([3], [3])])
+@pytest.mark.parametrize("cols", [8, 16])
+def test_a_window_wider_than_any_sequence_is_none(lib, rows, lens, window, cols):
+    """Rows in front of the first token have negative positions, from which such a window cannot be taken in 32 bits."""
+    visits, bad_rows, bad_pages = walk(lib, 16, rows, lens, 2, 1, window, 7, cols)
+    without, _, _ = walk(lib, 16, rows, lens, 2, 1, 0, 7, cols)
+    assert bad_rows == bad_pages == 0 and without.sum() > 0
+    np.testing.assert_array_equal(visits, without)
+
+
 def test_one_row_per_sequence_without_an_array(lib):
     visits, _, _ = walk(lib, 16, [1, 1, 1], [4, 90, 1], 4, 2, 0, 444, begin=None)
     assert visits.sum() == (4 + 90 + 1) * 8
