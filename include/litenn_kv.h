@@ -127,8 +127,9 @@ int qmm_kv_read(int device, const qmm_kv_cache* cache, const qmm_kv_batch* batch
  * h / (heads / kv_heads).  A row that sees no token gives zeros.  Tokens that a row does not see do not reach it,
  * whatever their pages hold.
  *   q [rows, heads * head_dim] of q_type, out the same shape of out_type.  fp32 results carry fp32's precision (scores
- *   and probabilities go through the tensor cores in two fp16 parts each); bf16 results of long prompts are computed
- *   with fp16 operands.
+ *   and probabilities go through the tensor cores in two fp16 parts each, probabilities times a block's scale relative
+ *   to the largest scale among the tokens: beside one that is 2^16 times as large, small values keep fewer bits); bf16
+ *   results of long prompts are computed with fp16 operands.
  *   workspace       QMM_KV_WORKSPACE_BYTES bytes, 256-byte aligned, zeroed once before their first use and left
  *                   zeroed where it matters by every call.  Calls that may run at the same time need one each.
  * Pointers are 16-byte aligned and strides whole multiples of 16 bytes; out may not overlap q.

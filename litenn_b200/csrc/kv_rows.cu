@@ -44,6 +44,7 @@ constexpr int JOIN = 8;  // parts that are loaded at once when a list entry's pa
 // Probabilities are taken as 2^4 .. 2^11 where the largest score lies: it may grow by SLACK before the sums are scaled down (every
 // other tile brings one of eight columns a new maximum), and fp16 parts of small ones keep their bits.
 constexpr float BIAS = 4.0f, SLACK = 7.0f;
+constexpr float MOST_P = 16.0f;  // and are multiplied by this much at most: 2^15
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p)
 {
@@ -489,7 +490,7 @@ __global__ void __launch_bounds__(RowsShape<FMT, HD, NT>::WARPS * 32, RowsShape<
         const int key_scale_at = kv_scale_place(HD, g, 0);  // of token g; token g + 8 and block b are a constant away
         const int reach = a.window > 0 ? a.window - 1 : 0x7FFFFFFF;  // a row at pos sees pos - reach .. pos
         float o[NT][HD / 16][4] = {};
-        float vs = 0.0f;      // power of two that brings value scales near one
+        float vs = 0.0f;      // power of two that brings value scales near one; up to MOST_P of it goes into the probabilities
         uint32_t limit = 0;   // fp16 bits: scales above it lower vs
         constexpr int U = kv_unit(FMT), LANE = kv_lane_bytes(FMT, HD), VEC = kv_vec(FMT, HD), VB = VEC / U;  // blocks of a vector
         constexpr int BP = VB % 2 == 0 ? 2 : 1;                                                                 // and those multiplied in turn
@@ -676,7 +677,10 @@ __global__ void __launch_bounds__(RowsShape<FMT, HD, NT>::WARPS * 32, RowsShape<
                     }
                     if (QUANT) {
                         // probabilities times scales stay within fp16: `vs` is set by the first tile's largest scale and
-                        // lowered when a later one may be above `limit`, so what fp16 rounds away is relative to the largest
+                        // lowered when a later one may be above `limit`, so what fp16 rounds away is relative to the largest.
+                        // What of it the probabilities have no room for (scales below 2^-5) multiplies the scales, exactly: without
+                        // that the second parts of small values lie below fp16's last bit (512 tokens of Q8_0 values of size 0.001
+                        // were off by 2e-5 of their norm)
                         load_words<(QUANT ? 2 * NB : 1) * 4>(d, vbase + PLANE + t * 2 * NB * 4);
                         if (!WHOLE) {
                             uint32_t any[2] = {0, 0};
@@ -713,7 +717,7 @@ __global__ void __launch_bounds__(RowsShape<FMT, HD, NT>::WARPS * 32, RowsShape<
                                 all = fmaxf(all, __shfl_xor_sync(0xFFFFFFFFu, all, sh));
                             }
                             // 2^11 of probability, 2^5 of room: the joined bits of scales of one size stay below it
-                            const int e = max(-17, min(4, -1 - ilogbf(fmaxf(fminf(all, 65504.0f), 0x1p-24f))));
+                            const int e = max(-17, min(19, -1 - ilogbf(fmaxf(fminf(all, 65504.0f), 0x1p-24f))));
                             const float now = vs == 0.0f ? scalbnf(1.0f, e) : fminf(vs, scalbnf(1.0f, e + 4));
                             if (vs != 0.0f && now != vs) {
                                 const float down = now / vs;
@@ -730,6 +734,14 @@ __global__ void __launch_bounds__(RowsShape<FMT, HD, NT>::WARPS * 32, RowsShape<
                             }
                             vs = now;
                             limit = __half_as_ushort(__float2half_rz(fminf(16.0f / now, 65504.0f)));
+                        }
+                        if (vs > MOST_P) {
+                            const __half2 up = __float2half2_rn(vs * (1.0f / MOST_P));  // at most 2^15
+#pragma unroll
+                            for (int i2 = 0; i2 < 2 * NB; ++i2) {
+                                uint32_t& w2 = d[i2 % (QUANT ? 2 * NB : 1)];
+                                w2 = h2_bits(__hmul2(as_h2(w2), up));
+                            }
                         }
                     } else if (!WHOLE) {
                         // tokens that not every column sees are kept out of the product, whose operand all columns share
@@ -773,7 +785,8 @@ __global__ void __launch_bounds__(RowsShape<FMT, HD, NT>::WARPS * 32, RowsShape<
                     for (int n = 0; n < NT; ++n) {
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
-                            const float2 pj = QUANT ? make_float2(s[n][2 * u + j].x * vs, s[n][2 * u + j].y * vs) : s[n][2 * u + j];
+                            const float in_p = fminf(vs, MOST_P);
+                            const float2 pj = QUANT ? make_float2(s[n][2 * u + j].x * in_p, s[n][2 * u + j].y * in_p) : s[n][2 * u + j];
                             const __half2 up = __floats2half2_rn(pj.x, pj.y);
                             const float2 f = __half22float2(up);
                             ph[n][j] = as_h2(transpose8(h2_bits(up)) & (QUANT || WHOLE ? 0xFFFFFFFFu : all_see[j]));

@@ -128,3 +128,14 @@ def norm_bound(hd, q_size, k_size, half_operands):
     probabilities and values by 2^-11 each.  Twice the sum: an upper bound with room for the maxima."""
     score = 2 * 2.0 ** -11 * q_size * k_size * hd ** 0.5 * hd ** -0.5
     return 2.0 ** -8 + 2 * (score + 2 * 2.0 ** -11 if half_operands else 2.0 ** -19)
+
+
+def fp32_norm_bound(score_size):
+    """2-norm of an fp32 result's error over the result's, scores of standard deviation `score_size` (natural logarithms).
+    An error of a score is one of its probability, and independent ones of all tokens pass into the result with the weights that
+    the values themselves have.  A score is a sum over hd / 32 blocks, each of four products on the tensor cores (two steps of
+    16 dimensions, q's two fp16 parts) whose running sum is cut at 2^-23 of itself; codes with their offset are 2.4 times as
+    large as without, and a block's sum is score_size / (hd / 32)^(1/2): together 2 * 2.4 * 2^-23 score_size, with the blocks'
+    sums in fp32 2^-20.5 score_size.  exp2, the two parts of a probability and of its product with a scale: 2^-21.
+    Four times the sum, for what is not independent and for the largest of many."""
+    return 4 * (score_size * 2.0 ** -20.5 + 2.0 ** -21)

@@ -449,6 +449,23 @@ def test_large_and_small_magnitudes(fmt):
         assert np.abs(got - want).max() <= ref.attention_bound(q, kk, vv, hd ** -0.5, False)
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("size", [100.0, 1.0, 1e-2, 1e-3, 1e-4, 1e-5])
+@pytest.mark.parametrize("hd,heads,n", [(64, 4, 20), (64, 32, 700), (128, 4, 500), (128, 24, 2500), (96, 4, 333), (256, 4, 90)])
+def test_fp32_results_carry_fp32_s_precision(fmt, size, hd, heads, n):
+    """In the 2-norm, whatever the size of the values: scales of blocks down to fp16's smallest."""
+    rng = np.random.default_rng(32)
+    p = Paged(fmt, 1, hd, 16, [n])
+    k = rng.standard_normal((n, 1, hd)).astype(np.float32)
+    v = (rng.standard_normal((n, 1, hd)) * size).astype(np.float32)
+    kd, vd = torch_of(k), torch_of(v)
+    p.cache.append(p.batch([n], [n]), None, 0, 0, 0, 0, kd.data_ptr(), hd, vd.data_ptr(), hd, 0, 0, 0)
+    q = (rng.standard_normal((3, heads, hd)) * 2).astype(np.float32)
+    got = p.attend(q, [3], [n], heads)
+    want = ref.attention(q, ref.stored(k, fmt), ref.stored(v, fmt), n, hd ** -0.5)
+    assert np.linalg.norm(want) > 0 and np.linalg.norm(got - want) <= np.linalg.norm(want) * ref.fp32_norm_bound(2.0)
+
+
 def test_padding_rows_and_strided_rows_stay_as_they_were():
     import torch
     rng = np.random.default_rng(11)
