@@ -666,6 +666,32 @@ def test_prompts_whose_scores_grow_along_the_keys():
 
 
 @pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("n,below,sink_value", [(3000, 10.0, 0.0), (3000, 20.6, 0.0), (3000, 24.4, 0.0), (40000, 20.4, 0.01), (40000, 24.4, 0.01)])
+@pytest.mark.parametrize("last", [False, True])
+def test_prompts_with_a_long_tail_below_one_key(fmt, n, below, sink_value, last):
+    """One key that takes nearly all of the probability and has hardly a value, before or behind many that are alike."""
+    rng = np.random.default_rng(33)
+    hd, heads, rows = 64, 2, 150
+    p = Paged(fmt, 1, hd, 16, [n])
+    k = np.zeros((n, 1, hd), np.float32)
+    v = (np.abs(rng.standard_normal((n, 1, hd))) + 0.5).astype(np.float32)
+    at = n - rows if last else 0
+    k[at], v[at] = 1.0, sink_value
+    kd, vd = torch_of(k), torch_of(v)
+    p.cache.append(p.batch([n], [n]), None, 0, 0, 0, 0, kd.data_ptr(), hd, vd.data_ptr(), hd, 0, 0, 0)
+    kk, vv = ref.stored(k, fmt)[:, 0], ref.stored(v, fmt)[:, 0]
+    scale = np.float32(below * np.log(2) / kk[at].sum())  # queries of ones
+    got = p.attend(np.ones((rows, heads, hd), np.float32), [rows], [n], heads, out_bf16=True, prompt=True, scale=float(scale))
+    w = np.exp2(np.float64(scale) * kk.sum(-1) / np.log(2) - below)[:, None]
+    total, mass = np.cumsum(w, 0)[n - rows:], np.cumsum(w * vv, 0)[n - rows:]
+    want = (mass / total)[:, None]
+    # bf16's half step; fp16 of a probability and of a value; half of fp16's last bit, 2^-32.75 of the largest, for every key.  A
+    # maximum behind the tail scales the sums that were there down, in fp32
+    bound = want * (2.0 ** -8 + 2 * 2.0 ** -11 + 2.0 ** -18) + n * 2.0 ** -32.75 * vv.max()
+    assert (np.abs(got - want) <= bound).all(), (np.abs(got - want) / want).max()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
 def test_prompts_what_a_row_does_not_see_does_not_reach_it(fmt):
     rng = np.random.default_rng(22)
     n, rows, hd, heads = 400, 200, 128, 2
