@@ -125,11 +125,12 @@ int qmm_kv_read(int device, const qmm_kv_cache* cache, const qmm_kv_batch* batch
  * Attention of the rows over their sequences' pages: out = softmax(scale * q . K) V over the tokens at or before the
  * row's position (the last `window` of them if window > 0).  `heads` query heads share kv_heads, head h reads kv head
  * h / (heads / kv_heads).  A row that sees no token gives zeros.  Tokens that a row does not see do not reach it,
- * whatever their pages hold.
+ * whatever their pages hold.  A value that is not finite (in quants its block of 32) makes its dimensions of the rows that
+ * see it infinite or NaN, and no others.
  *   q [rows, heads * head_dim] of q_type, out the same shape of out_type.  fp32 results carry fp32's precision (scores
  *   and probabilities go through the tensor cores in two fp16 parts each, probabilities times a block's scale relative
- *   to the largest scale among the tokens: beside one that is 2^16 times as large, small values keep fewer bits); bf16
- *   results of long prompts are computed with fp16 operands.
+ *   to the largest scale among the tokens: a value 2^-k of the largest keeps 28 - k bits); bf16 results of long prompts
+ *   are computed with fp16 operands.
  *   workspace       QMM_KV_WORKSPACE_BYTES bytes, 256-byte aligned, zeroed once before their first use and left
  *                   zeroed where it matters by every call.  Calls that may run at the same time need one each.
  * Pointers are 16-byte aligned and strides whole multiples of 16 bytes; out may not overlap q.

@@ -20,7 +20,7 @@
 // once, probabilities are fp16 relative to a maximum that may lag 2^8 behind (O is scaled only when it grows by more).  Each of
 // the four roundings is up to 2^-11 of its value where the bf16 result's own is up to 2^-8; probabilities below 2^-21 of the
 // largest are off by up to 2^-32.75 of it.  Sums are fp32.  A value that is not finite would reach every column of the product (0 times infinity): it enters as 0, and
-// the columns that see its token are made NaN.
+// its dimension is made NaN in the columns that see its token.
 #include <algorithm>
 #include <type_traits>
 
@@ -53,7 +53,7 @@ struct PromptShape {
     static constexpr int Q_BYTES = PANELS * M_TILE * 128;      // of an M tile
     static constexpr int K_BYTES = PANELS * BLOCK * 128;       // of a stage
     static constexpr int V_BYTES = BLOCK / 64 * HD * 128;
-    static constexpr int CONTROL = 4096;                       // barriers and what the warps tell one another
+    static constexpr int CONTROL = 8192;                       // barriers and what the warps tell one another
     static constexpr int SMEM = 1024 + CONTROL + 2 * Q_BYTES + 2 * K_BYTES + 2 * V_BYTES;
 };
 
@@ -75,6 +75,7 @@ struct Control {
     int late;
     uint32_t poison[8][KV_TILES];  // of the last blocks, per tile: tokens whose value is not finite
     float q_scale[COLS];
+    uint32_t odd[4][COLS];         // dimensions in which a column sees a value that is not finite: bit d of word n is 32 n + d
 };
 
 // Instruction descriptor: D fp32, A and B fp16, both K-major, M = 128, N = n.
@@ -209,6 +210,11 @@ __device__ __forceinline__ void quants(const uint32_t* w, uint32_t (&v)[4])
             v[i] = w[i];
         }
     }
+}
+// Two fp16, those that are not finite made 0.
+__device__ __forceinline__ uint32_t finite_or_0(uint32_t x)
+{
+    return ((x & 0x7C00u) == 0x7C00u ? 0u : x & 0xFFFFu) | ((x & 0x7C000000u) == 0x7C000000u ? 0u : x & 0xFFFF0000u);
 }
 // Volatile: the loads are issued where they stand (as plain ones they were moved down to their uses, a block later).
 template <int BYTES>
@@ -604,7 +610,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
                 }
                 if (ok) {
                     // tokens that no column sees, and values that are not finite, enter as 0
-                    uint32_t odd[2];
+                    uint32_t odd[2];  // tokens 2t, 2t + 1 of either half: some value of this lane's is not finite
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         __half2 sum = as_h2(0u);
@@ -641,7 +647,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
                             }
                         }
                     };
-                    if (__any_sync(0xFFFFFFFFu, (odd[0] | odd[1]) != 0) || edge) {
+                    const bool any_odd = __any_sync(0xFFFFFFFFu, (odd[0] | odd[1]) != 0);
+                    if (any_odd || edge) {
                         uint32_t keep[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
@@ -659,8 +666,18 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
                                 for (int tt = 0; tt < 4; ++tt) {
                                     poison |= (who >> tt & 1u) << (8 * j + 2 * tt + e);
                                 }
-                                if (!seen || (who >> t & 1u)) {
+                                if (!seen) {
                                     keep[j] &= ~half;
+                                }
+                            }
+                        }
+                        if (any_odd) {
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                                for (int n = 0; n < (QUANT ? NB : LANE / 4); ++n) {
+                                    uint32_t& x = QUANT ? vs[j][n % (QUANT ? NB : 1)] : vw[j][n % (LANE / 4)];
+                                    x = finite_or_0(x);
                                 }
                             }
                         }
@@ -692,19 +709,38 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
             const int pos = it.first_pos + (it.col0 + c) / a.group;
             const int low = kv_first_seen(pos, a.window);
             float m = -INFINITY, l = 0.0f;
-            bool ok = true, poisoned = false;
+            bool ok = true;
             const int my_blocks = it.blocks[i];
-            // whether this column sees a value of block kb that is not finite.  The block's words stay for eight blocks, and
-            // the warps that write them are at most two ahead of the values that are multiplied
+            // The dimensions in which this column sees a value of block kb that is not finite.  The words that name its tokens stay for
+            // eight blocks, and the warps that write them are at most two ahead of the values that are multiplied; the dimensions
+            // come from the cache, one to a lane.  In shared memory: four registers for them took 5 % of a long prompt's time.
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                ctl.odd[n][c] = 0;
+            }
             auto look_for_poison = [&](int kb) {
                 const uint32_t mine =
                     lane < KV_TILES ? *reinterpret_cast<volatile uint32_t*>(&ctl.poison[(blocks_before + kb) & 7][lane]) : 0u;
                 if (__any_sync(0xFFFFFFFFu, mine != 0)) {
                     for (int w = 0; w < KV_TILES; ++w) {
-                        const uint32_t bits = __shfl_sync(0xFFFFFFFFu, mine, w);
-                        for (int k = 0; bits != 0 && k < KV_TILE; ++k) {
-                            const int key = it.k0 + kb * BLOCK + w * KV_TILE + k;
-                            poisoned |= (bits >> k & 1u) && key <= pos && key >= low;
+                        const int tok0 = it.k0 + kb * BLOCK + w * KV_TILE;
+                        const uint8_t* values = nullptr;
+                        for (uint32_t bits = __shfl_sync(0xFFFFFFFFu, mine, w); bits != 0; bits &= bits - 1) {
+                            if (!values) {  // the tile's page has been looked up before: it is the pool's
+                                values = a.pool.base + kv_tile_index(a.pool, max(kv_page(a.pool, a.seqs, it.seq, tok0), 0), it.head, tok0) * TILE +
+                                         PLANE + SCALES;
+                            }
+                            const int k = __ffs(bits) - 1;
+                            const bool sees = tok0 + k <= pos && tok0 + k >= low;
+#pragma unroll 1
+                            for (int n = 0; n < NB; ++n) {
+                                const uint8_t* x = QUANT ? values + PLANE + kv_scale_place(HD, k, n)
+                                                         : values + kv_place(FMT, HD, k >> 3, (lane & ~3) + (k >> 1 & 3), n, 4 * (lane & 3) + 2 * (k & 1));
+                                const uint32_t bad = __ballot_sync(0xFFFFFFFFu, (*reinterpret_cast<const uint16_t*>(x) & 0x7C00u) == 0x7C00u);
+                                if (sees) {
+                                    ctl.odd[n][c] |= bad;
+                                }
+                            }
                         }
                     }
                 }
@@ -834,7 +870,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
             // bytes of 32 rows at a time took 3 us an item.
             uint8_t* place = q_smem + i * Shape::Q_BYTES + (c % M_TILE) * 128;
             const bool none = my_blocks == 0 || (m == -INFINITY && l == 0.0f);
-            const float inv = none ? 0.0f : poisoned ? __uint_as_float(0x7FC00000u) : 1.0f / l;
+            const float inv = none ? 0.0f : 1.0f / l;
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
                 float o[2][16];
@@ -858,6 +894,13 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
                         *reinterpret_cast<uint4*>(place + n / 2 * (M_TILE * 128) + (((n % 2 * 4 + k) ^ (c & 7)) << 4)) =
                             make_uint4(x[0], x[1], x[2], x[3]);
                     }
+                }
+            }
+#pragma unroll 1
+            for (int n = 0; n < NB; ++n) {
+                for (uint32_t odd = ctl.odd[n][c]; odd != 0; odd &= odd - 1) {
+                    const int d = __ffs(odd) - 1;
+                    *reinterpret_cast<uint16_t*>(place + n / 2 * (M_TILE * 128) + (((n % 2 * 4 + d / 8) ^ (c & 7)) << 4) + d % 8 * 2) = 0x7FC0u;
                 }
             }
             __syncwarp();

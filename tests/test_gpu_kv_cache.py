@@ -713,6 +713,30 @@ def test_prompts_what_a_row_does_not_see_does_not_reach_it(fmt):
 
 
 @pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("hd,window", [(128, 100), (64, 0)])
+def test_prompts_a_value_that_is_not_finite_stays_in_its_dimension(fmt, hd, window):
+    """Quants: in its block of 32.  The other dimensions of the rows that see it are what they are without it."""
+    rng = np.random.default_rng(34)
+    n, rows, heads = 400, 200, 2
+    p = Paged(fmt, 1, hd, 16, [n])
+    k = rng.standard_normal((n, 1, hd)).astype(np.float32)
+    v = rng.standard_normal((n, 1, hd)).astype(np.float32)
+    v[330, 0, hd - 58], v[20, 0, 1], v[399, 0, hd - 1], v[210, 0, 0], v[331, 0, 33] = np.inf, np.nan, -np.inf, np.nan, np.inf
+    if window == 0:
+        v[20, 0, 1], v[210, 0, 0] = 0.0, 0.0  # every row would see them
+    kd, vd = torch_of(k), torch_of(v)
+    p.cache.append(p.batch([n], [n]), None, 0, 0, 0, 0, kd.data_ptr(), hd, vd.data_ptr(), hd, 0, 0, 0)
+    q = rng.standard_normal((rows, heads, hd)).astype(np.float32)
+    got = p.attend(q, [rows], [n], heads, out_bf16=True, prompt=True, window=window)
+    kk, vv = ref.stored(k, fmt), ref.stored(v, fmt)
+    odd = ~np.isfinite(ref.attention(q, kk, vv, n, hd ** -0.5, window))
+    assert odd.any() and not odd.all()
+    np.testing.assert_array_equal(~np.isfinite(got), odd)
+    want = ref.attention(q, kk, np.where(np.isfinite(vv), vv, 0), n, hd ** -0.5, window)
+    assert np.linalg.norm((got - want)[~odd]) <= np.linalg.norm(want[~odd]) * ref.norm_bound(hd, 1.0, 1.0, True)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
 def test_prompts_rows_that_see_nothing_and_padding(fmt):
     rng = np.random.default_rng(23)
     p = Paged(fmt, 1, 64, 16, [30, 0])
