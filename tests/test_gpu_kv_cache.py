@@ -421,6 +421,27 @@ def test_what_a_row_does_not_see_does_not_reach_it(fmt, rows):
             assert np.abs(got - want)[~sees].max() <= bound
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("size", [1.0, 1e-2])
+def test_a_token_of_nan_leaves_other_rows_their_precision(fmt, size):
+    """The first tile that the call sees holds one token that the first row alone sees, and nothing of its value is a number."""
+    rng = np.random.default_rng(35)
+    n, hd, heads, rows, window = 213, 64, 4, 3, 100
+    p = Paged(fmt, 1, hd, 16, [n])
+    k = rng.standard_normal((n, 1, hd)).astype(np.float32)
+    v = (rng.standard_normal((n, 1, hd)) * size).astype(np.float32)
+    first = n - rows - window + 1
+    assert first % 16 == 15
+    v[first] = np.nan
+    kd, vd = torch_of(k), torch_of(v)
+    p.cache.append(p.batch([n], [n]), None, 0, 0, 0, 0, kd.data_ptr(), hd, vd.data_ptr(), hd, 0, 0, 0)
+    q = (rng.standard_normal((rows, heads, hd)) * 2).astype(np.float32)
+    got = p.attend(q, [rows], [n], heads, window=window)
+    want = ref.attention(q, ref.stored(k, fmt), ref.stored(v, fmt), n, hd ** -0.5, window)
+    assert np.isnan(got[0]).all() and np.isnan(want[0]).all()
+    assert np.linalg.norm(got[1:] - want[1:]) <= np.linalg.norm(want[1:]) * ref.fp32_norm_bound(2.0)
+
+
 def test_a_row_of_nothing_but_nan_is_nan():
     rng = np.random.default_rng(7)
     p = Paged(ref.Q4_0, 1, 64, 16, [700, 10])
