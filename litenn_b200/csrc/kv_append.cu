@@ -89,7 +89,8 @@ __device__ __forceinline__ float quantize4(const float (&x)[4], int lane, uint32
         if (FMT == FMT_Q4_0) {
             q[i] = __float_as_uint(__fadd_rd(fminf(fmaxf(__fadd_rn(y, 8.5f), 0.0f), 15.0f), 8388608.0f)) & 15u;
         } else {
-            const uint32_t r = __float_as_uint(__fadd_rd(fminf(__fadd_rn(fabsf(y), 0.5f), 127.0f), 8388608.0f)) & 127u;
+            // half added rounding down: to the nearest, 0.5 - 2^-25 would become 1
+            const uint32_t r = __float_as_uint(__fadd_rd(fminf(__fadd_rd(fabsf(y), 0.5f), 127.0f), 8388608.0f)) & 127u;
             q[i] = y < 0.0f ? 128u - r : 128u + r;
         }
         q[i] = odd ? (FMT == FMT_Q4_0 ? 8u : 128u) : q[i];

@@ -333,6 +333,30 @@ def test_values_that_no_block_holds_among_many_rows(fmt):
     assert int(np.isnan(want).sum()) == 3 * 32
 
 
+@pytest.mark.parametrize("n", [3, 900])
+def test_q8_0_rounds_half_away_from_zero(n):
+    """Halves, and the numbers next to them: 0.5 - 2^-25 plus a half is 1 in fp32, and its nearest whole number is 0."""
+    import torch
+    hd = 64
+    v = np.zeros((n, 1, hd), np.float32)
+    v[:, 0, 0], v[:, 0, 32] = 127.0, -127.0  # scales of 1
+    halves = np.array([0.5, 1.5, 2.5, 62.5, 63.5, 126.5], np.float32)
+    below, above = np.nextafter(halves, np.float32(0)), np.nextafter(halves, np.float32(200))
+    x = np.concatenate([halves, below, above])
+    v[:, 0, 1:19], v[:, 0, 33:51] = x, -x
+    want = np.concatenate([halves + 0.5, halves - 0.5, halves + 0.5])
+    p = Paged(ref.Q8_0, 1, hd, 16, [n])
+    xd = torch_of(v.reshape(n, hd))
+    b = p.batch([n], [n])
+    p.cache.append(b, None, 0, 0, 0, 0, xd.data_ptr(), hd, xd.data_ptr(), hd, 0, 0, 0)
+    out = torch.empty(2, n, hd, device="cuda")
+    p.cache.read(b, out[0].data_ptr(), hd, out[1].data_ptr(), hd, 0)
+    assert capi.kernel_status(0) == 0
+    for o in np_of(out):
+        np.testing.assert_array_equal(o[:, 1:19], np.tile(want, (n, 1)))
+        np.testing.assert_array_equal(o[:, 33:51], np.tile(-want, (n, 1)))
+
+
 # ---- attention -----------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("fmt", FMTS)
