@@ -237,6 +237,13 @@ __device__ __forceinline__ RowPlace find_row(const KvPool& c, const KvSeqs& b, i
             if (__ldg(b.row_begin + s) <= row && row < __ldg(b.row_begin + s + 1)) {
                 atomicMin(found, s);
             }
+            if (row == 0) {  // what cannot be right may have no rows
+                bool bad;
+                kv_seq(c, b, s, bad);
+                if (bad) {
+                    atomicExch(b.status, KV_BAD_ROWS);
+                }
+            }
         }
     }
     __syncthreads();

@@ -998,6 +998,22 @@ def test_bad_pages_and_rows_among_many_rows(fmt):
     assert torch.equal(p.pool, pool)
 
 
+@pytest.mark.parametrize("n", [8, 900])
+def test_sequences_that_cannot_be_right_are_reported_without_rows_of_their_own(n):
+    import torch
+    hd = 64
+    p = Paged(ref.Q8_0, 1, hd, 16, [n, n, n])
+    x = torch_of(np.ones((n, hd), np.float32))
+    back = torch.zeros(2, n, hd, device="cuda")
+    for begin, lens in (([0, 4, 2, 2], [n] * 3), ([0, 4, n + 1, n + 1], [n] * 3), ([0, 4, 4, -1], [n] * 3), ([-1, -1, 0, n], [n] * 3),
+                        ([0, n, n, n], [n, -1, n]), ([0, n, n, n], [n, n, p.width * 16 + 1])):
+        b = p.batch([n], lens)
+        t = torch.tensor(begin, dtype=torch.int32, device="cuda")
+        b.row_begin_dev = t.data_ptr()
+        assert "22" in status_of(lambda: p.cache.append(b, None, 0, 0, 0, 0, x.data_ptr(), hd, x.data_ptr(), hd, 0, 0, 0))
+        assert "22" in status_of(lambda: p.cache.read(b, back[0].data_ptr(), hd, back[1].data_ptr(), hd, 0))
+
+
 def test_empty_calls_do_nothing():
     p = Paged(ref.Q4_0, 1, 64, 16, [4])
     b = capi.KVBatch(0, p.width, p.table_dev.data_ptr(), p.table_dev.data_ptr(), 0, 0)
