@@ -75,6 +75,11 @@ int check_batch(const char* who, const qmm_kv_cache* c, const qmm_kv_batch* b)
     if (b->batch > 0 && (!b->kv_len_dev || (b->table_width > 0 && !b->page_table_dev))) {
         return fail("%s: page_table or kv_len is null", who);
     }
+    for (const int32_t* p : {b->page_table_dev, b->kv_len_dev, b->row_begin_dev}) {
+        if (reinterpret_cast<uintptr_t>(p) % sizeof(int32_t) != 0) {
+            return fail("%s: page_table, kv_len or row_begin is not 4-byte aligned", who);
+        }
+    }
     if (!b->row_begin_dev && b->batch > b->rows) {
         return fail("%s: %d sequences have one row each, but there are %lld rows", who, b->batch, (long long)b->rows);
     }

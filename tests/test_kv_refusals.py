@@ -77,6 +77,14 @@ def test_batches(call):
     refused(lambda: call(cache(page=65536), b=batch(width=1 << 15)), text="31 bits")
 
 
+@pytest.mark.parametrize("call", [attend, append])
+def test_arrays_of_whole_numbers_are_aligned(call):
+    for off in (1, 2, 3):
+        refused(lambda: call(b=batch(table=A + off)), text="4-byte aligned")
+        refused(lambda: call(b=batch(length=A + off)), text="4-byte aligned")
+        refused(lambda: call(b=batch(begin=A + off)), text="4-byte aligned")
+
+
 def test_attention_arguments():
     refused(lambda: attend(heads=0))
     refused(lambda: attend(heads=5), text="divide")
