@@ -69,7 +69,7 @@ struct Item {
 };
 
 struct Control {
-    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2][2], o_full;  // probabilities: of either half of the keys
+    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2][2], o_full, drained;  // probabilities: of either half of the keys
     uint32_t tmem;
     Item item[2];                  // the one that is worked on and the next; seq < 0: there is none
     int late;
@@ -255,6 +255,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
             g_mbar_init(&ctl.p_full[i][1], 4);
         }
         g_mbar_init(&ctl.o_full, 1);
+        g_mbar_init(&ctl.drained, 1);
         ctl.late = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -928,6 +929,13 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
     __syncthreads();
     if (mma_warp) {
         fence_after();
+        if (ctl.late) {  // products may still be under way: once more, before their operands' and their sums' memory is given back
+            if (elect_one()) {
+                umma_commit(&ctl.drained);
+            }
+            __syncwarp();
+            g_mbar_wait_warp(&ctl.drained, 0);
+        }
         __syncwarp();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
         // the last CTA leaves the counters zeroed for the next call

@@ -506,10 +506,20 @@ __global__ void __launch_bounds__(RowsShape<FMT, HD, NT>::WARPS * 32, RowsShape<
             const unsigned int have = have_all >> (i * STEP & 31) & ((1u << STEP) - 1);
             if (have != 0 && !late) {
                 late = !__all_sync(0xFFFFFFFFu, mbar_wait(&my_bars[slot], phases >> slot & 1u));
-                phases ^= 1u << slot;
-                if (late && lane == 0) {
-                    atomicExch(a.seqs.status, KV_LATE_COPY);
+                if (late) {
+                    // no copy is started from here on; those in flight (of this step and of the next ones) are waited for once
+                    // more, so that they do not land in what the ring's place is used for
+                    if (lane == 0) {
+                        atomicExch(a.seqs.status, KV_LATE_COPY);
+                    }
+                    for (int k = 0; k < DEPTH && i + k < my_steps; ++k) {
+                        const bool same = ((i + k) ^ i) < AHEAD;
+                        if (((same ? have_all : have_next) >> ((i + k) * STEP & 31) & ((1u << STEP) - 1)) != 0) {
+                            mbar_wait(&my_bars[(i + k) % DEPTH], phases >> ((i + k) % DEPTH) & 1u);
+                        }
+                    }
                 }
+                phases ^= 1u << slot;
             }
             // Two copies of what is done: whole steps, and single tiles, which pay for masks: those where columns differ in what
             // they see, and a last one that has no second.
