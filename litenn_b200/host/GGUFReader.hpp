@@ -12,7 +12,8 @@
 //     size" otherwise); every failure is a std::runtime_error.
 // LoadPackedWeight feeds a quantized tensor's payload straight into the upload-time repack
 // (PackedWeight, LiteNNQuantMatMul.hpp), so the file-to-HBM path never dequantizes; DequantizeOnDevice
-// is the fp32 route for tensors in a block format without matmul kernels.
+// is the fp32 route for tensors in a block format without matmul kernels.  ParseRopeScaling says how the
+// file's rotary positions are stretched.
 #pragma once
 
 #include <cuda_runtime_api.h>
@@ -28,6 +29,7 @@
 #include <vector>
 
 #include "LiteNNQuantMatMul.hpp"
+#include "../../include/litenn_kv.h"
 
 namespace LiteNN
 {
@@ -175,6 +177,14 @@ namespace GGUF
 		}
 	};
 
+	// How a file's rotary positions are stretched past the trained context: what qmm_llama_set_rope_scaling and
+	// qmm_rope_frequencies (litenn_kv.h) take.
+	struct RopeScaling
+	{
+		qmm_rope_scaling scaling{ QMM_ROPE_SCALE_NONE, 1.0f, 0.0f, 32.0f, 1.0f };
+		std::vector<float> frequencyFactors; // rope_freqs.weight, one per pair of dimensions; empty: the file has none
+	};
+
 	class Archive
 	{
 	public:
@@ -275,6 +285,55 @@ namespace GGUF
 			h.ropeDimensionCount = FindMetadata(p + "rope.dimension_count") ? Unsigned(p + "rope.dimension_count")
 			                                                               : h.HeadDimension();
 			return h;
+		}
+
+		// The keys `<arch>.rope.scaling.*` (or the older `<arch>.rope.scale_linear`) and the tensor rope_freqs.weight.  A file
+		// that is stretched in a way the kernels do not know is refused: run unscaled it would answer wrongly.
+		RopeScaling ParseRopeScaling()
+		{
+			RopeScaling r;
+			const std::string p = String("general.architecture") + ".rope.", q = p + "scaling.";
+			const std::string type = FindMetadata(q + "type") ? String(q + "type") : "none";
+			if (type == "linear" || type == "yarn")
+			{
+				r.scaling.kind = type == "yarn" ? QMM_ROPE_SCALE_YARN : QMM_ROPE_SCALE_LINEAR;
+				r.scaling.factor = static_cast<float>(Real(q + "factor"));
+			}
+			else if (type != "none")
+			{
+				throw std::runtime_error("GGUF rope scaling '" + type + "' is not supported (none, linear, yarn)");
+			}
+			else if (FindMetadata(p + "scale_linear"))
+			{
+				r.scaling.factor = static_cast<float>(Real(p + "scale_linear"));
+				r.scaling.kind = r.scaling.factor == 1.0f ? QMM_ROPE_SCALE_NONE : QMM_ROPE_SCALE_LINEAR;
+			}
+			if (r.scaling.kind == QMM_ROPE_SCALE_YARN)
+			{
+				r.scaling.trained = static_cast<float>(FindMetadata(q + "original_context_length")
+				                                           ? Unsigned(q + "original_context_length")
+				                                           : Unsigned(String("general.architecture") + ".context_length"));
+				if (FindMetadata(q + "yarn_beta_fast"))
+				{
+					r.scaling.beta_fast = static_cast<float>(Real(q + "yarn_beta_fast"));
+				}
+				if (FindMetadata(q + "yarn_beta_slow"))
+				{
+					r.scaling.beta_slow = static_cast<float>(Real(q + "yarn_beta_slow"));
+				}
+			}
+			if (HasTensor("rope_freqs.weight"))
+			{
+				const auto& t = Tensor("rope_freqs.weight");
+				if (t.type != TensorType::F32 || t.shape.size() != 1)
+				{
+					throw std::runtime_error("GGUF tensor 'rope_freqs.weight' is not a row of fp32");
+				}
+				const auto payload = ReadPayload(t);
+				r.frequencyFactors.resize(payload.size() / sizeof(float));
+				std::memcpy(r.frequencyFactors.data(), payload.data(), payload.size());
+			}
+			return r;
 		}
 
 	private:
