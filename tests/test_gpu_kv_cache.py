@@ -906,6 +906,55 @@ def test_prompts_bad_pages_and_rows():
     assert int(p.workspace[:16384].to(torch.int32).sum()) == 0
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("appended", [300, 900])
+def test_the_last_positions_that_a_table_can_name(fmt, appended):
+    """Positions near 2^31: appended row by row or in tiles, attended by few rows and by a prompt, with a window."""
+    import torch
+    rng = np.random.default_rng(36)
+    hd, heads, page, width, window = 64, 4, 65536, 32766, 100
+    n = width * page - 20
+    pool = torch.zeros(capi.kv_pool_bytes(fmt, 1, hd, page, 1), dtype=torch.uint8, device="cuda")
+    cache = capi.KVCache(fmt, 1, hd, page, 1, pool.data_ptr())
+    table = torch.zeros(1, width, dtype=torch.int32, device="cuda")  # one page holds what is looked at
+    length = torch.tensor([n], dtype=torch.int32, device="cuda")
+    work = torch.zeros(capi.KV_WORKSPACE_BYTES, dtype=torch.uint8, device="cuda")
+
+    def batch(rows, total=None):
+        begin = torch.tensor([0, rows], dtype=torch.int32, device="cuda")
+        return capi.KVBatch(1, width, table.data_ptr(), length.data_ptr(), begin.data_ptr(), total or rows), begin
+
+    x = rng.standard_normal((appended, heads + 2, hd)).astype(np.float32)
+    xd, q_out = torch_of(x.reshape(appended, -1)), torch.zeros(appended, heads * hd, device="cuda")
+    freq, gain = capi.rope_frequencies(hd, 10000.0)
+    f = torch_of(freq)
+    at, stride = xd.data_ptr(), (heads + 2) * hd
+    b, hold = batch(appended)
+    cache.append(b, capi.Rope(hd, 0, f.data_ptr(), gain), heads, 0, at, stride, at + heads * hd * 4, stride, at + (heads + 1) * hd * 4,
+                 stride, q_out.data_ptr(), 0, heads * hd)
+    back = torch.zeros(2, appended, hd, device="cuda")
+    cache.read(b, back[0].data_ptr(), hd, back[1].data_ptr(), hd, 0)
+    assert capi.kernel_status(0) == 0
+    pos = np.arange(n - appended, n)
+    turned = ref.rotate(x[:, :heads + 1], pos, freq, gain, hd, False)
+    # both sides take the sine and the cosine of the same 64-bit angle: the results are the same but for fp32's last bit
+    np.testing.assert_allclose(np_of(q_out).reshape(appended, heads, hd), turned[:, :heads], rtol=2.0 ** -22, atol=2.0 ** -40)
+    np.testing.assert_array_equal(np_of(back)[1], ref.stored(x[:, heads + 1], fmt).astype(np.float32))
+    keys, vals = np_of(back)[0][:, None].astype(np.float64), np_of(back)[1][:, None].astype(np.float64)
+    assert np.linalg.norm(keys[:, 0] - ref.stored(turned[:, heads], fmt)) <= 1e-3 * np.linalg.norm(keys)  # a quant may be another
+    for rows, out_type, total in ((3, torch.float32, None), (150, torch.bfloat16, 1024)):
+        q = (rng.standard_normal((total or rows, heads, hd)) * 2).astype(np.float32)
+        qd, out = torch_of(q.reshape(len(q), -1)), torch.zeros(len(q), heads * hd, device="cuda", dtype=out_type)
+        b, hold = batch(rows, total)
+        cache.attend(b, heads, qd.data_ptr(), 0, heads * hd, out.data_ptr(), int(out_type == torch.bfloat16), heads * hd, hd ** -0.5,
+                     window, work.data_ptr())
+        assert capi.kernel_status(0) == 0
+        want = ref.attention(q[:rows], keys, vals, appended, hd ** -0.5, window)
+        bound = ref.fp32_norm_bound(2.0) if total is None else ref.norm_bound(hd, 2.0, 1.0, True)
+        got = np_of(out)[:rows].reshape(rows, heads, hd)
+        assert np.linalg.norm(got - want) <= np.linalg.norm(want) * bound
+
+
 # ---- what cannot be right is reported -------------------------------------------------------------------------------------
 
 def status_of(call):
