@@ -47,6 +47,14 @@ constexpr int KV_LATE_PROMPT = 24;             // a bounded wait ran out
 // room for more bits, and scales the sums more often: 512 rows behind 16384 tokens 341 us, with 2^6 348 us.
 constexpr float BIAS = 7.75f, SLACK = 8.0f;
 
+// A maximum (times its factor) whose rounding is not small beside BIAS and SLACK: of a score of 2^25 and its maximum the roundings
+// of the products are whole powers of two apart.  Such a column's scores lose the maximum before the factor.
+constexpr float FAR = 65536.0f;
+__device__ __forceinline__ bool is_far(float m)
+{
+    return fabsf(m) > FAR && m != -INFINITY;
+}
+
 template <int FMT, int HD>
 struct PromptShape {
     static constexpr int PANELS = HD / 64;                     // 64 dimensions: a 128-byte swizzle row
@@ -75,6 +83,7 @@ struct Control {
     int late;
     uint32_t poison[8][KV_TILES];  // of the last blocks, per tile: tokens whose value is not finite
     float q_scale[COLS];
+    float far_max[COLS];           // the running maximum before its factor, where that is past 2^16
     uint32_t odd[4][COLS];         // dimensions in which a column sees a value that is not finite: bit d of word n is 32 n + d
 };
 
@@ -711,6 +720,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
             const int low = kv_first_seen(pos, a.window);
             float m = -INFINITY, l = 0.0f;
             bool ok = true;
+            bool far = false;  // the maximum of some column of the warp has been past FAR
             const int my_blocks = it.blocks[i];
             // The dimensions in which this column sees a value of block kb that is not finite.  The words that name its tokens stay for
             // eight blocks, and the warps that write them are at most two ahead of the values that are multiplied; the dimensions
@@ -756,6 +766,38 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
                 fence_after();
                 // keys key0 + lo .. key0 + hi of the block are this column's
                 const int hi = pos - key0, lo = low - key0;
+                // Probabilities in a warp with a maximum past FAR: those columns' scores lose it before the factor
+                auto far_probabilities = [&]() {
+                    const float lost = is_far(m) ? ctl.far_max[c] : 0.0f;
+                    const float ref = is_far(m) ? -BIAS : m == -INFINITY ? 0.0f : m - BIAS;
+#pragma unroll 1
+                    for (int part = 0; part < BLOCK / 16; ++part) {
+                        float x[16];
+                        tmem_ld16(s_at + 16 * part, x);
+                        tmem_wait_ld(x);
+                        uint32_t p[8];
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) {
+                            const float e = exp2_fast(fmaf(x[k] - lost, qs, -ref));
+                            x[k] = 16 * part + k <= hi && 16 * part + k >= lo ? e : 0.0f;
+                            l += x[k];
+                        }
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            p[k] = h2_bits(__floats2half2_rn(x[2 * k], x[2 * k + 1]));
+                        }
+                        tmem_st8(s_at + 8 * part, p);  // over columns that have been read
+                        if (part == BLOCK / 32 - 1) {  // the first half of the product can begin
+                            tmem_wait_st();
+                            fence_before();
+                            __syncwarp();
+                            if (lane == 0) {
+                                g_mbar_arrive(&ctl.p_full[i][0]);
+                            }
+                        }
+                    }
+                    tmem_wait_st();
+                };
                 auto probabilities = [&](auto all_seen) {
                     constexpr bool WHOLE = decltype(all_seen)::value;
                     constexpr int PARTS = BLOCK / 16;
@@ -780,11 +822,19 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
                         tmem_wait_ld(s[(part + 1) & 1]);
                     }
                     float top = fmaxf(top4[0], max3(top4[1], top4[2], top4[3]));
+                    const float raw = top;
                     top = top == -INFINITY ? top : top * qs;
-                    const bool higher = top > m + SLACK || (m == -INFINITY && top > m);
+                    bool higher = top > m + SLACK || (m == -INFINITY && top > m);
+                    if (far && is_far(m)) {
+                        higher = raw > ctl.far_max[c] && (raw - ctl.far_max[c]) * qs > SLACK;
+                    }
                     if (__any_sync(0xFFFFFFFFu, higher)) {
-                        const float down = higher ? exp2_fast(m - top) : 1.0f;
-                        m = higher ? top : m;
+                        const float down = !higher ? 1.0f : exp2_fast(far && is_far(m) ? (ctl.far_max[c] - raw) * qs : m - top);
+                        if (higher) {
+                            m = top;
+                            ctl.far_max[c] = raw;
+                        }
+                        far = far || __any_sync(0xFFFFFFFFu, is_far(m));
                         l *= down;
                         if (kb > 0) {
                             float (&x)[16] = s[1];
@@ -800,6 +850,10 @@ __global__ void __launch_bounds__(THREADS, 1) kv_prompt_kernel(const KvAttnArgs 
                             }
                             tmem_wait_st();
                         }
+                    }
+                    if (far) {
+                        far_probabilities();
+                        return;
                     }
                     const float ref = m == -INFINITY ? 0.0f : m - BIAS;
                     static_assert(PARTS % 2 == 0, "the first part is in s[0] again");

@@ -420,11 +420,17 @@ __global__ void __launch_bounds__(RowsShape<FMT, HD, NT>::WARPS * 32, RowsShape<
             }
         }
 
-        // ---- queries: two fp16 parts of q * 2^e with the largest near 2^14, in operand order ----
+        // ---- queries: two fp16 parts of q * scale * log2(e) * 2^e with the largest near 2^14, in operand order.  With the scale in
+        // them the scores' factor is a power of two: a score and its maximum times that factor are exact, however large, where
+        // the roundings of other products would put whole powers of two between scores of 2^25 and their maximum ----
 #pragma unroll
         for (int n = 0; n < QC; ++n) {
             const int c = warp + n * WARPS;
             float (&v)[NB] = qv[n];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                v[b] *= a.scale * 1.44269504088896340736f;
+            }
             uint32_t bits = 0;  // magnitudes order as their bits; NaN above all
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
@@ -433,7 +439,7 @@ __global__ void __launch_bounds__(RowsShape<FMT, HD, NT>::WARPS * 32, RowsShape<
             bits = __reduce_max_sync(0xFFFFFFFFu, bits);
             const int exponent = (int)(bits >> 23) - 127;  // of the largest, -127 for a subnormal
             const int e = bits == 0 || exponent == 128 ? 0 : max(-112, min(120, 14 - exponent));
-            const float up = __uint_as_float((uint32_t)(e + 127) << 23 | (a.scale < 0.0f ? 0x80000000u : 0u));
+            const float up = __uint_as_float((uint32_t)(e + 127) << 23);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 const float y = v[b] * up;
@@ -449,7 +455,7 @@ __global__ void __launch_bounds__(RowsShape<FMT, HD, NT>::WARPS * 32, RowsShape<
                 f[2 + ee] = high ? __hmul(lo, __float2half_rn(0.0625f)) : lo;
             }
             if (lane == 0) {
-                qscale[c] = fabsf(a.scale) * 1.44269504088896340736f * __uint_as_float((uint32_t)(127 - e) << 23) * (1.0f / KEY_UNIT<FMT>);
+                qscale[c] = __uint_as_float((uint32_t)(127 - e) << 23) * (1.0f / KEY_UNIT<FMT>);
             }
         }
         __syncthreads();
@@ -636,9 +642,10 @@ __global__ void __launch_bounds__(RowsShape<FMT, HD, NT>::WARPS * 32, RowsShape<
                         top.x = fmaxf(top.x, __shfl_xor_sync(0xFFFFFFFFu, top.x, sh));
                         top.y = fmaxf(top.y, __shfl_xor_sync(0xFFFFFFFFu, top.y, sh));
                     }
-                    top.x = top.x == -INFINITY ? top.x : fmaf(top.x, qs[n].x, -BIAS);  // a scale of 0 makes NaN of -inf
-                    top.y = top.y == -INFINITY ? top.y : fmaf(top.y, qs[n].y, -BIAS);
-                    const bool higher0 = top.x > m[n].x + SLACK, higher1 = top.y > m[n].y + SLACK;
+                    // rounded so that a probability stays below 2^(BIAS + SLACK) where these are lost in large sums
+                    top.x = __fmaf_ru(top.x, qs[n].x, -BIAS);
+                    top.y = __fmaf_ru(top.y, qs[n].y, -BIAS);
+                    const bool higher0 = top.x > __fadd_rd(m[n].x, SLACK), higher1 = top.y > __fadd_rd(m[n].y, SLACK);
                     if (__any_sync(0xFFFFFFFFu, higher0 || higher1)) {
                         const float down0 = higher0 ? exp2_fast(m[n].x - top.x) : 1.0f;  // 0 for the first
                         const float down1 = higher1 ? exp2_fast(m[n].y - top.y) : 1.0f;
@@ -662,7 +669,7 @@ __global__ void __launch_bounds__(RowsShape<FMT, HD, NT>::WARPS * 32, RowsShape<
                     }
                     if (!WHOLE) {
 #pragma unroll
-                        for (int j = 0; j < 2 * N; ++j) {  // also where qs is 0
+                        for (int j = 0; j < 2 * N; ++j) {  // also in a column that has seen nothing yet but NaN
                             const int pos = tok0 + 8 * j + g;
                             s[n][j].x = pos <= pos_of[n][0] && pos >= pos_of[n][0] - reach ? s[n][j].x : 0.0f;
                             s[n][j].y = pos <= pos_of[n][1] && pos >= pos_of[n][1] - reach ? s[n][j].y : 0.0f;

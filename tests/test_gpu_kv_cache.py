@@ -511,6 +511,35 @@ def test_fp32_results_carry_fp32_s_precision(fmt, size, hd, heads, n):
     assert np.linalg.norm(want) > 0 and np.linalg.norm(got - want) <= np.linalg.norm(want) * ref.fp32_norm_bound(2.0)
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("size", [1e3, 1e5, 1e6, 1e8, 1e20])
+def test_scores_of_any_size(fmt, prompt, size):
+    """One key takes all: scores past 2^24, whose last bits are whole powers of two of a probability."""
+    rng = np.random.default_rng(37)
+    n, rows, heads, hd = 300, 150, 4, 64
+    p = Paged(fmt, 1, hd, 16, [n])
+    k = (rng.standard_normal((n, 1, hd)) * np.linspace(0.5, 2, n)[:, None, None]).astype(np.float32)  # maxima come late, too
+    v = rng.standard_normal((n, 1, hd)).astype(np.float32)
+    kd, vd = torch_of(k), torch_of(v)
+    p.cache.append(p.batch([n], [n]), None, 0, 0, 0, 0, kd.data_ptr(), hd, vd.data_ptr(), hd, 0, 0, 0)
+    kk, vv = ref.stored(k, fmt)[:, 0], ref.stored(v, fmt)[:, 0]
+    q = (rng.standard_normal((rows, heads, hd)) * size).astype(np.float32)
+    got = p.attend(q, [rows], [n], heads, out_bf16=prompt, prompt=prompt)
+    score = np.einsum("rhd,nd->rhn", q.astype(np.float64), kk) * hd ** -0.5
+    score[np.arange(n)[None, None] > (n - rows + np.arange(rows))[:, None, None] + np.zeros((1, heads, 1))] = -np.inf
+    first, second = np.sort(score, -1)[..., -1], np.sort(score, -1)[..., -2]
+    # with fp16 operands (the prompt kernel's) each product is off by up to 2^-10 of itself, for two keys of at most 16: 2^-5 of q's
+    # magnitudes; and e^-40 is nothing
+    assert np.abs(kk).max() < 16
+    clear = (first - second > 2.0 ** -5 * np.abs(q).sum(-1) * hd ** -0.5) & (first - second > 40)
+    assert clear.mean() > 0.5 or size < 1e4
+    want = vv[score.argmax(-1)]
+    assert np.isfinite(got).all()
+    bound = np.abs(want) * (2.0 ** -8 + 2.0 ** -10 if prompt else 2.0 ** -20) + 1e-15
+    assert (np.abs(got - want) <= bound)[clear].all()
+
+
 def test_padding_rows_and_strided_rows_stay_as_they_were():
     import torch
     rng = np.random.default_rng(11)
