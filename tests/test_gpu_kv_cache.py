@@ -540,6 +540,23 @@ def test_scores_of_any_size(fmt, prompt, size):
     assert (np.abs(got - want) <= bound)[clear].all()
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("scale", [0.0, -0.125, 1.0, 1e-20])
+def test_scales_of_any_sign_and_size(fmt, prompt, scale):
+    """0 and 1e-20: the mean of what a row sees."""
+    rng = np.random.default_rng(38)
+    n, rows, heads, hd = 200, 130, 4, 64
+    p = Paged(fmt, 2, hd, 16, [n])
+    ks, vs = p.fill(rng)
+    q = rng.standard_normal((rows, heads, hd)).astype(np.float32)
+    got = p.attend(q, [rows], [n], heads, out_bf16=prompt, prompt=prompt, scale=scale, window=150)
+    want = ref.attention(q, ks[0], vs[0], n, np.float64(np.float32(scale)), 150)
+    size = abs(scale) * hd ** 0.5  # of the scores
+    bound = 2.0 ** -8 + 4 * 2.0 ** -11 * (size + 1) if prompt else ref.fp32_norm_bound(size)
+    assert np.linalg.norm(got - want) <= np.linalg.norm(want) * bound
+
+
 def test_padding_rows_and_strided_rows_stay_as_they_were():
     import torch
     rng = np.random.default_rng(11)
