@@ -59,7 +59,7 @@ typedef struct qmm_kv_cache {
 
 /* Which rows of a call belong to which sequence, and where the sequence's tokens are.  Row i of the n rows of
  * sequence s is the token at position kv_len[s] - n + i: kv_len counts the rows of the call.
- * The arrays are read on the device when the call runs, so a captured call sees their values at replay.  What
+ * The arrays (4-byte aligned) are read on the device when the call runs, so a captured call sees their values at replay.  What
  * cannot be right (a page outside the pool, rows outside the tensors, a length outside the table) is skipped and
  * reported through qmm_kernel_status: 21 a page, 22 rows or a length. */
 typedef struct qmm_kv_batch {
@@ -133,6 +133,9 @@ int qmm_kv_read(int device, const qmm_kv_cache* cache, const qmm_kv_batch* batch
  *   are computed with fp16 operands.
  *   workspace       QMM_KV_WORKSPACE_BYTES bytes, 256-byte aligned, zeroed once before their first use and left
  *                   zeroed where it matters by every call.  Calls that may run at the same time need one each.
+ * Which kernel a call runs goes by its shape on the host: `rows` (all that the tensors have room for), heads and types, not by
+ * lengths.  bf16 results of many rows go to one that reads a sequence's tokens once for 256 rows times heads, and does not
+ * split them: long histories of few rows, single tokens above all, belong in a call of their own.
  * Pointers are 16-byte aligned and strides whole multiples of 16 bytes; out may not overlap q.
  */
 int qmm_kv_attention(int device, const qmm_kv_cache* cache, const qmm_kv_batch* batch, int heads, const void* q_dev,

@@ -544,10 +544,12 @@ __device__ __forceinline__ void turn_halves(const KvAppendArgs& a, const double2
 
 // Many rows.  blockIdx.x: groups of kv heads, then groups of query heads; blockIdx.y: tiles.  A warp takes a row at a time.  A whole
 // tile is put together in shared memory: stored from the registers, its two- and four-byte pieces made a sector of DRAM traffic
-// each.  Bound: 1999 rows of 32 heads of 128 with as many kv heads, fp32 to Q4_0, move 170 MB in 64 us (41 % of the copy rate) with half of the issue
-// slots taken: rotation and its conversions in fp64, and the blocks' quants.  Sixteen prompts of 33 to 901 rows, 64 query and 8 kv
-// heads of 128, half of each rotated, bf16 to fp16: 124 us (42 %).  Registers for three CTAs of an SM: two left loads exposed (218 us), four
-// spill (144 us).  Sixteen warps a CTA: 64 and 147 us.
+// each.  1999 rows of 32 heads of 128 with as many kv heads, fp32 to Q4_0, are 140 MB in 47 us (46 % of the copy rate), to Q8_0 148 MB
+// in 51, to fp16 164 MB in 46; sixteen prompts of 33 to 901 rows, 64 query and 8 kv heads of 128, half of each rotated, bf16 to fp16,
+// 306 MB in 105 us (44 %).  Bound: latency, at 4.8 warps a scheduler (half of the issue slots, 7 % of the fp64 units): a tile's place, its
+// angles and a barrier come before the first rows are asked for.  With the read of the same rows behind it (42 MB in 20 us, 61 MB in 21):
+// registers for three CTAs of an SM 64 and 124 us, two left loads exposed (ragged prompts 218), four spill (144); sixteen warps a CTA 64
+// and 147.
 template <int FMT, int HD, bool HALVES>
 __global__ void __launch_bounds__(TILE_WARPS * 32, 24 / TILE_WARPS) kv_append_tile_kernel(const KvAppendArgs a)
 {
@@ -822,6 +824,7 @@ cudaError_t read_tiles_fmt(const KvReadArgs& a, cudaStream_t stream)
 // A row's CTA is done sooner, a tile's does less work.  8 kv heads of 128, Q4_0, 32 query heads, rows / tiles: append of one
 // sequence of 400 rows 12.6 / 16.0 us, 1000 rows 20.8 / 21.1 us (fp16 18.3 / 13.1), 2000 rows 38.8 / 25.1 us, 8000 rows 156 / 66 us;
 // of 500 sequences of 4 rows 39.6 / 51.3 us; read of 1000 rows 6.3 / 6.2 us, of 8000 rows 33.8 / 16.8 us.
+// The rule goes by rows, not by heads or formats: fp16 would cross earlier.
 bool by_tiles(const KvSeqs& b)
 {
     return b.rows >= 800 && b.rows >= (int64_t)8 * b.batch && tiles_of(b) <= 65535;

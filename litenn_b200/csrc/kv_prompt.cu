@@ -11,8 +11,9 @@
 //
 // Bound: the chain of a block.  A column's softmax takes about 3000 cycles of 128 keys (128 exponentials and maxima of one thread,
 // TMEM loads between them), the two products 1700, and with two M tiles in turn a block takes 2.5 us.  512 rows of 64 heads (8 kv heads of
-// 128, Q4_0) behind 16384 tokens: 338 us, 827 TFLOP/s, 51 % of the measured dense peak.  1999 rows of 32 heads from the start: 86 us;
-// an item costs 8 us beside its blocks (queries 4, results 2, first keys 2) and has 9 of them on average.
+// 128, Q4_0) behind 16384 tokens: 347 us, 804 TFLOP/s, 50 % of the measured dense peak.  1999 rows of 32 heads from the start: 83 us;
+// an item costs 8 us beside its blocks (queries 4, results 2, first keys 2) and has 9 of them on average.  Nothing splits the keys of an
+// item: 64 rows of 64 heads behind 131072 tokens are 16 items, 1024 blocks each, and take 2.5 ms (floor 0.17).
 // Tried and slower (the first of the two cases): blocks of 64 keys with two score buffers 471 us where 128 took 358; one warp fewer for
 // keys and values, the tiles dealt in turn, 460; a softmax in one pass over chunks with a running maximum 452.
 //
@@ -1047,6 +1048,8 @@ cudaError_t launch_prompt_fmt(const KvAttnArgs& a, int sm_count, cudaStream_t st
 // rows kernel cuts anything over the whole GPU.  2000 tokens of 128 dimensions, rows / prompt kernel, Q4_0: one sequence of 32 rows
 // of 64 heads 43 / 56 us, of 64 rows 69 / 56 us; of 64 rows of 32 heads (one to a kv head) 43 / 49 us, of 128 rows 68 / 51 us; eight
 // sequences of 4 rows of 64 heads 44 / 49 us, of 8 rows 69 / 49 us, of 16 rows of 32 heads (16 columns each) 70 / 102 us.
+// What the rule does not know are the lengths, which are the device's, and which rows are whose: a prompt of 512 rows of 64 heads and 31 single
+// tokens behind 1023 others take 80 us in one call and 75 in two, behind 8191 324 and 150, behind 65535 2266 and 716.
 bool kv_takes_prompt(const KvAttnArgs& a)
 {
     return a.out_type == QMM_OUT_BF16 && (a.pool.head_dim == 64 || a.pool.head_dim == 128) && a.seqs.row_begin != nullptr &&

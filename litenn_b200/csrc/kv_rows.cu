@@ -19,10 +19,13 @@
 // transposes per tile that turn the scores' layout (row = token) into the probabilities' operand layout (row = column).
 //
 // What bounds it beside the bytes: instructions, about 415 a warp for a Q4_0 tile of 128 dimensions (57 % of the issue
-// slots, 3.6 warps a scheduler), and 12 to 15 us of a call that its length does not change (the lengths' scan 1.5, queries and pages 3, joining warps
-// and CTAs 3 to 5).  One token, us: 131072 tokens of 8 kv heads of 128 in Q4_0, 64 heads 61 (2.5 TB/s; its copies alone 45), 16 sequences of
-// 700 to 8191 tokens 44, 639 tokens of 32 kv heads 14; 16 sequences of 500 to 2000 tokens of 32 kv heads in fp16 63 (5.2 TB/s, 79 %
-// of the copy rate); 8 sequences of 100 to 4000 tokens in Q8_0, 3 to 5 rows each of 32 heads, 28.
+// slots, 3.6 warps a scheduler), and what a call takes beside its tiles: 5 us where every entry is one CTA's, 12 to 15 where entries are
+// shared (the lengths' scan 1.5, queries and pages 3, joining warps and CTAs 3 to 5).  One token, us: 131072 tokens of 8 kv heads of 128,
+// 64 heads, in Q4_0 61 (2.5 TB/s; its copies alone 45), in Q8_0 80 (floor 44); 16 sequences of 700 to 8191 tokens in Q4_0 44, in Q8_0 53;
+// 639 tokens of 32 kv heads 15; 16 sequences of 500 to 2000 tokens of 32 kv heads in fp16 64 (5.1 TB/s, 79 % of the copy rate); 8 sequences
+// of 100 to 4000 tokens in Q8_0, 3 to 5 rows each of 32 heads, 28.  Prompts come here too where the prompt kernel does not take them
+// (fp32 results, heads of 96 and 256), a pass over all their keys for every 8 or 16 columns: 1999 rows of 32 heads of 128 with fp32
+// results 606 us, of 32 heads of 96 490, of 16 heads of 256 655, where the prompt kernel takes 83 for 128 dimensions.
 //
 // Work is cut evenly (kv_rows_plan.cuh) on the device, from the lengths, so that ragged batches and single long sequences both
 // fill the GPU and a captured launch follows the lengths.  Where a list entry spans CTAs, each leaves its part in the workspace
@@ -203,7 +206,8 @@ struct RowsShape {
     // have a handful each, 45.3 / 49.3 us).  Where the sums take 64 registers one leaves room for more CTAs (16 columns of 64, 8
     // sequences of 2000 tokens, 26.6 / 31.8 us), and fp16 has no scales to share (64 dimensions, 131072 tokens 52.8 / 57.4 us).
     static constexpr int STEP = NT == 1 && HD <= 128 && FMT != KV_F16 ? 2 : 1;
-    // CTAs per SM, by the registers the sums take (NT * HD / 4 of them)
+    // CTAs per SM, by the registers the sums take (NT * HD / 4 of them); at four, with 128 registers a thread, the 128-wide Q4_0 form
+    // spills 16 bytes, the 96-wide fp16 one 48
     static constexpr int BY_REGISTERS = NT * HD <= 128 ? 4 : NT * HD <= 256 ? 3 : 1;
     static constexpr int DEPTH = 2;  // steps in the ring; three were no faster (131072 tokens, 64/8 heads, Q4_0: 62.8 us, two 60.9)
     static constexpr int QFRAG = NT * HD / 16 * 32 * 16;  // query operand registers
