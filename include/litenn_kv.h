@@ -29,7 +29,8 @@
  * A value is q * scale.  Blocks are made as GGUF makes them, in fp32: Q4_0 d = m / -8 where m is the value of
  * largest magnitude (the first of equals), q + 8 = min(15, floor(x * (1 / d) + 8.5)); Q8_0 d = max|x| / 127, q =
  * x * (1 / d) rounded half away from zero.  |d| is held to 8188 and 515.5, so that every value lies within fp16's
- * range (larger ones saturate); a block with an infinity or a NaN gets a NaN scale and reads as NaN.
+ * range (larger ones saturate); a block with an infinity or a NaN gets a NaN scale and reads as NaN.  An fp16 cache holds
+ * values rounded to fp16: past its range they are infinities.
  */
 #ifndef LITENN_KV_H
 #define LITENN_KV_H
