@@ -20,8 +20,8 @@
 // Numerics: queries are brought to fp16 by a power of two per row, keys and values are the cache's q * scale rounded to fp16
 // once, probabilities are fp16 relative to a maximum that may lag 2^8 behind (O is scaled only when it grows by more).  Each of
 // the four roundings is up to 2^-11 of its value where the bf16 result's own is up to 2^-8; probabilities below 2^-21 of the
-// largest are off by up to 2^-32.75 of it.  Sums are fp32.  A value that is not finite would reach every column of the product (0 times infinity): it enters as 0, and
-// its dimension is made NaN in the columns that see its token.
+// largest are off by up to 2^-32.75 of it.  Sums are fp32.  A value that is not finite would reach every column of the product
+// (0 times infinity): it enters as 0, and its dimension is made NaN in the columns that see its token.
 #include <algorithm>
 #include <type_traits>
 
